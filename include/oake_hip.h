@@ -24,6 +24,8 @@
  *   image.resize((w/1.5, h/1.5))      oadp/oake/blocks.py:72-76 -> oake_resize_u8
  *   Dataset._preprocess (blocks)      oadp/oake/blocks.py:54-109 -> oake_blocks_batch (pyramid + every block
  *                                                             crop of a whole flush of images)
+ * and, on the logits of crops against label embeddings (or of any vocabulary), without a counterpart there:
+ * oake_token_logprobs, oake_distill_top_logits and their backward passes.
  *
  * Conventions: plain C, int status (0 = OAKE_OK), no exception crosses the ABI.  All data
  * pointers named d_* are DEVICE pointers owned by the caller (e.g. a torch tensor's
@@ -67,7 +69,10 @@ enum {
   OAKE_F32 = 0,
   OAKE_F16 = 1,
   OAKE_BF16 = 2,
-  OAKE_U8 = 3
+  OAKE_U8 = 3,
+  /* index lists (oake_token_logprobs, oake_distill_top_logits) */
+  OAKE_I32 = 4,
+  OAKE_I64 = 5
 };
 /* Layout flag, OR-ed into the `out_dtype` of oake_crop_resize_normalize(_batch) and the `in_dtype` of oake_encode_objects on
  * a handle whose conv1 pads (objects mode: stride 16, padding 15 [REF oadp/oake/objects.py:298-301]): the crops are written
@@ -122,7 +127,8 @@ OAKE_API void oake_default_config(oake_config* cfg);
 OAKE_API int oake_create(const oake_config* cfg, int device, oake_handle** out);
 OAKE_API void oake_destroy(oake_handle* h);
 
-/* Last error text for this handle (or for a failed oake_create when h == NULL). */
+/* Last error text for this handle (h == NULL: of the calling thread's last failed oake_create or entry point without a
+ * handle). */
 OAKE_API const char* oake_last_error(const oake_handle* h);
 
 /* Derived geometry: grid = (image + 2*padding - patch)/stride + 1, tokens = grid*grid + 1. */
@@ -288,6 +294,77 @@ OAKE_API int oake_jpeg_entropy_decode(const uint8_t* h_data, size_t nbytes, int1
 OAKE_API int oake_jpeg_reconstruct(oake_handle* h, const uint8_t* h_data, size_t nbytes, const int16_t* h_coefs,
                           size_t ncoefs, uint8_t* d_out_hwc, size_t out_capacity, int* height,
                           int* width, void* stream);
+
+/*
+ * Operators on logits: what a classifier over label embeddings (or a language model's head) answers, and what a student
+ * learns from it.  They take no handle: they run on the device that is current in the calling thread, on `stream`, keep no
+ * state between calls, allocate nothing and wait for nothing (they can be captured into a graph; two calls at once need a
+ * workspace each).  Errors: oake_last_error(NULL), per calling thread.
+ *
+ * Common to all four: d_logits is [rows, vocab] of `dtype` (OAKE_F32 | OAKE_F16 | OAKE_BF16), rows `row_stride` ELEMENTS
+ * apart (0: one row for all), elements next to each other; rows 0 .. 2^31 - 1 (0: nothing is done), vocab
+ * 1 .. 2^31 - 1.  z = scale * logit with 0 < scale < inf (CLIP's logit scale, 1 / temperature), p = softmax(z) over the
+ * allowed places; fp32 throughout, gradients rounded once to `dtype`.  Index lists are OAKE_I32 | OAKE_I64, contiguous;
+ * a negative index is padding.  An index >= vocab cannot be refused without waiting for the GPU: it is never
+ * followed, and makes what depends on it NaN.  All pointers are aligned to their element type.
+ *
+ * oake_logits_workspace: bytes of scratch the two forward entry points need for these sizes (often 0; `top` as passed
+ * there to oake_token_logprobs, 0 for oake_distill_top_logits).  The workspace is 16-byte aligned, needs no
+ * initialisation and is free again when the call's work on the stream is done.
+ */
+OAKE_API int oake_logits_workspace(int64_t rows, int64_t vocab, int dtype, int top, size_t* bytes);
+
+/*
+ * Per row: lse = log sum_allowed e^z; logprobs[t] = z[target t] - lse for n_targets (0 .. 1024) given tokens; entropy
+ * = -sum p log p; the `top` (0 .. 128) largest logits as log probabilities and int64 indices, best first, equal ones by
+ * the lowest index.  d_mask (or NULL): bytes, 0 = not allowed, rows mask_stride bytes apart (0: one mask of vocab bytes
+ * for all rows); whatever stands in a place that is not allowed is without effect.
+ *   a token that is not allowed, or whose logit is -inf     log probability -inf, and no alternative
+ *   fewer alternatives than `top`                            index -1, log probability -inf
+ *   a row with nothing allowed (or -inf everywhere)          lse -inf, entropy 0, log probabilities -inf
+ *   padding (a negative target)                              log probability 0
+ *   an allowed NaN or +inf                                   lse, entropy and log probabilities of the row are NaN;
+ *                                                            alternatives are ordered with NaN above all numbers
+ * d_lse, d_entropy, d_stats may be NULL.  d_stats [rows, 4] is what the backward pass needs of the forward one.
+ */
+OAKE_API int oake_token_logprobs(const void* d_logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                                 float scale, const uint8_t* d_mask, int64_t mask_stride, const void* d_targets,
+                                 int index_dtype, int n_targets, int top, float* d_logprobs, float* d_lse,
+                                 float* d_entropy, float* d_top_logprobs, int64_t* d_top_indices, float* d_stats,
+                                 void* d_workspace, size_t workspace_bytes, void* stream);
+/*
+ * d_grad [rows, vocab] of `dtype`, rows grad_stride elements apart (no overlap with each other or with the logits) =
+ * the gradient of sum(grad_logprobs * logprobs) + sum(grad_lse * lse) + sum(grad_entropy * entropy) + sum(grad_top *
+ * top_logprobs) with respect to the logits; each of the four (contiguous fp32, shaped as its output) may be NULL = 0.
+ * Places that are not allowed get 0, and a log probability of -inf is a constant (no gradient), as is padding.
+ */
+OAKE_API int oake_token_logprobs_backward(const void* d_logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                                          float scale, const uint8_t* d_mask, int64_t mask_stride, const void* d_targets,
+                                          int index_dtype, int n_targets, const int64_t* d_top_indices, int top,
+                                          const float* d_stats, const float* d_grad_logprobs, const float* d_grad_lse,
+                                          const float* d_grad_entropy, const float* d_grad_top, void* d_grad,
+                                          int64_t grad_stride, void* stream);
+
+/*
+ * A student's loss against a teacher's list: loss[row] = KL(q || p), p the softmax of the student's z.  The list
+ * (`top` 0 .. 1024 entries a row): d_top_indices and d_top_logprobs v (fp32; what oake_token_logprobs leaves in
+ * d_top_indices / d_top_logprobs), an entry with a negative index or v = -inf is absent; an index listed twice counts
+ * with both entries.
+ *   tail == 0   q = softmax of the row's entries (v up to a constant)
+ *   tail != 0   q = e^v, and all places outside the list are one bucket of probability max(0, 1 - sum q) (left out
+ *               where the student gives those places nothing at all)
+ * A row without entries: loss 0, gradient 0.  A listed place that the student gives probability 0: loss +inf, the
+ * gradient is the formula's.  NaN as above.  d_stats [rows, 8] is what the backward pass needs.
+ */
+OAKE_API int oake_distill_top_logits(const void* d_logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                                     float scale, const void* d_top_indices, int index_dtype, const float* d_top_logprobs,
+                                     int top, int tail, float* d_loss, float* d_stats, void* d_workspace,
+                                     size_t workspace_bytes, void* stream);
+/* d_grad = grad_loss[row] * d loss[row] / d logits; arguments as above and as in oake_token_logprobs_backward. */
+OAKE_API int oake_distill_top_logits_backward(const void* d_logits, int dtype, int64_t rows, int64_t vocab,
+                                              int64_t row_stride, float scale, const void* d_top_indices, int index_dtype,
+                                              const float* d_top_logprobs, int top, int tail, const float* d_stats,
+                                              const float* d_grad_loss, void* d_grad, int64_t grad_stride, void* stream);
 
 /*
  * Per-kernel timing with HIP events on the launch stream (bench.py's `roofline` object).

@@ -9,6 +9,7 @@ import pathlib
 OAKE_OK = 0
 OAKE_ERR_INVALID, OAKE_ERR_HIP, OAKE_ERR_STATE, OAKE_ERR_UNKNOWN_TENSOR, OAKE_ERR_UNSUPPORTED = 1, 2, 3, 4, 5
 OAKE_F32, OAKE_F16, OAKE_BF16, OAKE_U8 = 0, 1, 2, 3
+OAKE_I32, OAKE_I64 = 4, 5
 OAKE_LAYOUT_PADDED = 0x100
 OAKE_OPT_CLS_LAST, OAKE_OPT_GEMM_VARIANT, OAKE_OPT_GEMM_PANEL, OAKE_OPT_ATTENTION_VARIANT = 1, 2, 3, 4
 OAKE_OPT_PATCH_DIRECT = 5
@@ -36,6 +37,7 @@ class ProfileEntry(C.Structure):
 
 # name -> (restype, argtypes); every symbol include/oake_hip.h declares
 _VP, _I = C.c_void_p, C.c_int
+_LOGITS = [_VP, _I, C.c_int64, C.c_int64, C.c_int64, C.c_float]  # logits, dtype, rows, vocab, row_stride, scale
 SIGNATURES = {
     'oake_abi_version': (C.c_uint32, []),
     'oake_default_config': (None, [C.POINTER(OakeConfig)]),
@@ -68,6 +70,13 @@ SIGNATURES = {
     'oake_jpeg_entropy_decode': (_I, [_VP, C.c_size_t, _VP, C.c_size_t, C.POINTER(C.c_size_t)]),
     'oake_jpeg_reconstruct': (_I, [_VP, _VP, C.c_size_t, _VP, C.c_size_t, _VP, C.c_size_t, C.POINTER(C.c_int), C.POINTER(C.c_int), _VP]),
     'oake_decode_jpeg': (_I, [_VP, _VP, C.c_size_t, _VP, C.c_size_t, C.POINTER(C.c_int), C.POINTER(C.c_int), _VP]),
+    'oake_logits_workspace': (_I, [C.c_int64, C.c_int64, _I, _I, C.POINTER(C.c_size_t)]),
+    'oake_token_logprobs': (_I, [*_LOGITS, _VP, C.c_int64, _VP, _I, _I, _I, _VP, _VP, _VP, _VP, _VP, _VP, _VP,
+                                 C.c_size_t, _VP]),
+    'oake_token_logprobs_backward': (_I, [*_LOGITS, _VP, C.c_int64, _VP, _I, _I, _VP, _I, _VP, _VP, _VP, _VP, _VP,
+                                          _VP, C.c_int64, _VP]),
+    'oake_distill_top_logits': (_I, [*_LOGITS, _VP, _I, _VP, _I, _I, _VP, _VP, _VP, C.c_size_t, _VP]),
+    'oake_distill_top_logits_backward': (_I, [*_LOGITS, _VP, _I, _VP, _I, _I, _VP, _VP, _VP, C.c_int64, _VP]),
     'oake_profile_enable': (_I, [_VP, _I]),
     'oake_profile_read': (_I, [_VP, C.POINTER(ProfileEntry), _I, C.POINTER(_I)]),
     'oake_profile_reset': (_I, [_VP]),

@@ -24,6 +24,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import _lib
+from .logits import TokenLogprobs, label_logits, token_logprobs
 from .preprocess import Preprocess
 from .settings import settings
 
@@ -800,6 +801,15 @@ class CLIP:
     def encode_image(self, image: torch.Tensor, **kwargs) -> torch.Tensor:
         # reference: self.visual(image.type(self.dtype)); the cast happens inside the im2col kernel
         return self.visual(image, **kwargs)
+
+    def classify(self, image: torch.Tensor, labels: torch.Tensor, *, targets: torch.Tensor | None = None, top: int = 5,
+                 mask: torch.Tensor | None = None, scale: float = 100.0) -> TokenLogprobs:
+        """Zero-shot answers for a batch of crops: the ``top`` labels of each with their log probabilities, those of
+        ``targets``, the entropy.  ``labels`` [n, embed]: label embeddings (``oadp_amd.prompts.vild``), on the crops'
+        device; ``mask``: the labels that may be answered (a dataset's own, the base ones, ...); ``scale``: CLIP's logit
+        scale.  See ``oadp_amd.clip.logits.token_logprobs`` for shapes and special cases."""
+        embeddings = self.encode_image(image, normalize=True, out_dtype=torch.float32)
+        return token_logprobs(label_logits(embeddings, labels), targets, top=top, mask=mask, scale=scale)
 
     def eval(self) -> 'CLIP':
         return self

@@ -308,6 +308,14 @@ int upload_16(oake_handle* h, void* dst, const float* src, size_t numel) {
 
 }  // namespace
 
+int oake::fail_without_handle(int code, const char* text) noexcept {
+  try {
+    g_create_error = text;
+  } catch (...) {  // (out of memory: the status says enough)
+  }
+  return code;
+}
+
 extern "C" {
 
 uint32_t oake_abi_version(void) { return OAKE_ABI_VERSION; }

@@ -16,6 +16,9 @@
 
 namespace oake {
 
+// records the text of a failed entry point that has no handle (oake_last_error(NULL), per thread); returns `code`
+int fail_without_handle(int code, const char* text) noexcept;
+
 // 16-bit operand type selector (matches OAKE_F16 / OAKE_BF16 in include/oake_hip.h)
 enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2, DT_U8 = 3 };
 
