@@ -85,16 +85,21 @@ def _workspace_bytes(rows: int, vocab: int, dtype: int, top: int) -> int:
     return n.value
 
 
+# the current stream of a device as the C entries take it (the public call builds a Stream object: 1.1 us against 0.1,
+# where a whole call takes about 15)
+_current_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _launch(x: torch.Tensor, name: str, *args) -> None:
     """``name``(..., stream) with x's device current and its current stream."""
-    lib, dev = _lib.load(), x.device.index
-    stream = torch.cuda.current_stream(dev).cuda_stream
+    lib, dev = _lib.load(), x.get_device()
     if torch.cuda.current_device() == dev:
-        rc = getattr(lib, name)(*args, stream)
+        rc = getattr(lib, name)(*args, _current_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = getattr(lib, name)(*args, stream)
-    if rc != _lib.OAKE_OK:
+            rc = getattr(lib, name)(*args, _current_stream(dev))
+    if rc:
         _lib.check(lib, None, rc, name)
 
 
@@ -102,62 +107,66 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def _logits_args(x: torch.Tensor, scale: float) -> tuple:
-    return x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], x.stride(0), scale
-
-
-def _index_args(ids: torch.Tensor | None) -> tuple:
-    return (None, 0) if ids is None else (ids.data_ptr(), _INDEX[ids.dtype])
-
-
-def _workspace(x: torch.Tensor, top: int) -> tuple[torch.Tensor | None, int]:
-    n = _workspace_bytes(x.shape[0], x.shape[1], _DTYPES[x.dtype], top)
-    return (torch.empty(n, dtype=torch.uint8, device=x.device), n) if n else (None, 0)
-
-
 def _f32(g: torch.Tensor | None) -> torch.Tensor | None:
-    return None if g is None else g.to(torch.float32).contiguous()
+    if g is None or (g.dtype is torch.float32 and g.is_contiguous()):
+        return g
+    return g.to(torch.float32).contiguous()
+
+
+def _workspace(x: torch.Tensor, rows: int, vocab: int, dtype: int, top: int) -> tuple[torch.Tensor | None, int]:
+    n = _workspace_bytes(rows, vocab, dtype, top)
+    return (x.new_empty(n, dtype=torch.uint8), n) if n else (None, 0)
 
 
 def _score(x, targets, mask, mask_stride, top, scale, stats):
-    rows, dev = x.shape[0], x.device
-    n = 0 if targets is None else targets.shape[1]
-    logprobs = None if targets is None else torch.empty((rows, n), dtype=torch.float32, device=dev)
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
-    lse = torch.empty(rows, dtype=torch.float32, device=dev)
-    top_lp = torch.empty((rows, top), dtype=torch.float32, device=dev) if top else None
-    top_ids = torch.empty((rows, top), dtype=torch.int64, device=dev) if top else None
-    ws, nbytes = _workspace(x, top)
-    _launch(x, 'oake_token_logprobs', *_logits_args(x, scale), _ptr(mask), mask_stride, *_index_args(targets), n, top,
-            _ptr(logprobs), lse.data_ptr(), entropy.data_ptr(), _ptr(top_lp), _ptr(top_ids), _ptr(stats), _ptr(ws), nbytes)
+    (rows, vocab), dtype, f32 = x.shape, _DTYPES[x.dtype], torch.float32
+    logprobs = top_lp = top_ids = None
+    n = index = 0
+    if targets is not None:
+        n, index = targets.shape[1], _INDEX[targets.dtype]
+        logprobs = x.new_empty((rows, n), dtype=f32)
+    entropy, lse = x.new_empty(rows, dtype=f32), x.new_empty(rows, dtype=f32)
+    if top:
+        top_lp, top_ids = x.new_empty((rows, top), dtype=f32), x.new_empty((rows, top), dtype=torch.int64)
+    ws, nbytes = _workspace(x, rows, vocab, dtype, top)
+    _launch(x, 'oake_token_logprobs', x.data_ptr(), dtype, rows, vocab, x.stride(0), scale, _ptr(mask), mask_stride,
+            _ptr(targets), index, n, top, _ptr(logprobs), lse.data_ptr(), entropy.data_ptr(), _ptr(top_lp), _ptr(top_ids),
+            _ptr(stats), _ptr(ws), nbytes)
     return logprobs, entropy, lse, top_lp, top_ids
+
+
+def _differentiable_once(backward):
+    """``once_differentiable`` where a graph of the backward pass is asked for, without its cost where it is not."""
+    guarded = once_differentiable(backward)
+    return staticmethod(lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads))
 
 
 class _TokenLogprobs(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, targets, mask, mask_stride, top, scale):
-        stats = torch.empty((x.shape[0], 4), dtype=torch.float32, device=x.device)
+        stats = x.new_empty((x.shape[0], 4), dtype=torch.float32)
         out = _score(x, targets, mask, mask_stride, top, scale, stats)
         ctx.save_for_backward(x, targets, mask, out[4], stats)
         ctx.more = mask_stride, top, scale
         ctx.set_materialize_grads(False)
-        if out[4] is not None:
+        if top:
             ctx.mark_non_differentiable(out[4])
         return out
 
-    @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, g_logprobs, g_entropy, g_lse, g_top, _):
         x, targets, mask, top_ids, stats = ctx.saved_tensors
         mask_stride, top, scale = ctx.more
         if g_logprobs is None and g_entropy is None and g_lse is None and g_top is None:
             return (None,) * 6
         g_logprobs, g_entropy, g_lse, g_top = _f32(g_logprobs), _f32(g_entropy), _f32(g_lse), _f32(g_top)
-        grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        _launch(x, 'oake_token_logprobs_backward', *_logits_args(x, scale), _ptr(mask), mask_stride, *_index_args(targets),
-                0 if targets is None else targets.shape[1], _ptr(top_ids), top, stats.data_ptr(), _ptr(g_logprobs),
-                _ptr(g_lse), _ptr(g_entropy), _ptr(g_top), grad.data_ptr(), x.shape[1])
+        rows, vocab = x.shape
+        grad = x.new_empty((rows, vocab))
+        n, index = (0, 0) if targets is None else (targets.shape[1], _INDEX[targets.dtype])
+        _launch(x, 'oake_token_logprobs_backward', x.data_ptr(), _DTYPES[x.dtype], rows, vocab, x.stride(0), scale,
+                _ptr(mask), mask_stride, _ptr(targets), index, n, _ptr(top_ids), top, stats.data_ptr(), _ptr(g_logprobs),
+                _ptr(g_lse), _ptr(g_entropy), _ptr(g_top), grad.data_ptr(), vocab)
         return grad, None, None, None, None, None
 
 
@@ -206,33 +215,34 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     return TokenLogprobs(logprobs, entropy, lse, top_lp, top_ids)
 
 
-def _distill(x, ids, v, scale, tail, stats):
-    loss = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
-    ws, nbytes = _workspace(x, 0)
-    _launch(x, 'oake_distill_top_logits', *_logits_args(x, scale), ids.data_ptr(), _INDEX[ids.dtype], v.data_ptr(),
-            ids.shape[1], tail, loss.data_ptr(), stats.data_ptr(), _ptr(ws), nbytes)
-    return loss
+def _distill(x, ids, v, scale, tail):
+    (rows, vocab), dtype = x.shape, _DTYPES[x.dtype]
+    loss, stats = x.new_empty(rows, dtype=torch.float32), x.new_empty((rows, 8), dtype=torch.float32)
+    ws, nbytes = _workspace(x, rows, vocab, dtype, 0)
+    _launch(x, 'oake_distill_top_logits', x.data_ptr(), dtype, rows, vocab, x.stride(0), scale, ids.data_ptr(),
+            _INDEX[ids.dtype], v.data_ptr(), ids.shape[1], tail, loss.data_ptr(), stats.data_ptr(), _ptr(ws), nbytes)
+    return loss, stats
 
 
 class _DistillTopLogits(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, ids, v, scale, tail):
-        stats = torch.empty((x.shape[0], 8), dtype=torch.float32, device=x.device)
-        loss = _distill(x, ids, v, scale, tail, stats)
+        loss, stats = _distill(x, ids, v, scale, tail)
         ctx.save_for_backward(x, ids, v, stats)
         ctx.more = scale, tail
         return loss
 
-    @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, g_loss):
         x, ids, v, stats = ctx.saved_tensors
         scale, tail = ctx.more
         g_loss = _f32(g_loss)
-        grad = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        _launch(x, 'oake_distill_top_logits_backward', *_logits_args(x, scale), ids.data_ptr(), _INDEX[ids.dtype],
-                v.data_ptr(), ids.shape[1], tail, stats.data_ptr(), g_loss.data_ptr(), grad.data_ptr(), x.shape[1])
+        rows, vocab = x.shape
+        grad = x.new_empty((rows, vocab))
+        _launch(x, 'oake_distill_top_logits_backward', x.data_ptr(), _DTYPES[x.dtype], rows, vocab, x.stride(0), scale,
+                ids.data_ptr(), _INDEX[ids.dtype], v.data_ptr(), ids.shape[1], tail, stats.data_ptr(), g_loss.data_ptr(),
+                grad.data_ptr(), vocab)
         return grad, None, None, None, None
 
 
@@ -266,13 +276,14 @@ def distill_top_logits(logits: torch.Tensor, top_indices: torch.Tensor, top_logp
         raise ValueError('the teacher gets no gradient: detach() its top_logprobs')
     _check_same_device(logits, top_indices=top_indices, top_logprobs=top_logprobs)
     x = _as_rows(logits)
-    ids = top_indices.reshape(x.shape[0], k).contiguous()
-    v = top_logprobs.detach().reshape(x.shape[0], k).to(torch.float32).contiguous()
+    ids, v = top_indices, top_logprobs.detach() if top_logprobs.requires_grad else top_logprobs
+    if len(lead) != 1:
+        ids, v = ids.reshape(x.shape[0], k), v.reshape(x.shape[0], k)
+    ids, v = ids.contiguous(), _f32(v)
     if x.requires_grad and torch.is_grad_enabled():
         loss = _DistillTopLogits.apply(x, ids, v, scale, tail)
     else:
-        stats = torch.empty((x.shape[0], 8), dtype=torch.float32, device=x.device)
-        loss = _distill(x, ids, v, scale, tail, stats)
+        loss, _ = _distill(x, ids, v, scale, tail)
     return loss if len(lead) == 1 else loss.view(lead)
 
 

@@ -9,6 +9,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <type_traits>
 
 #include "../../include/oake_hip.h"
 #include "common.h"
@@ -36,6 +37,7 @@ __device__ __forceinline__ uint64_t place_key(float x, uint32_t j) {
   return (uint64_t)order_key(x) << 32 | (0xFFFFFFFFu - j);
 }
 
+
 struct Rows {  // rows of logits and what of them is allowed
   const void* x;
   int64_t rows, vocab, stride;
@@ -43,39 +45,177 @@ struct Rows {  // rows of logits and what of them is allowed
   int64_t mask_stride;   // 0: one mask for all rows
   float scale;
 };
-template <typename T>
-__device__ __forceinline__ float logit(const T* x, const uint8_t* mask, int64_t j) {
-  return mask && !mask[j] ? -kInf : (float)x[j];
-}
+struct Split {           // a row as `parts` chunks of `chunk` places, each a workgroup's (or a wave's) own
+  int64_t chunk;
+  int parts;
+};
 
 __device__ __forceinline__ int64_t load_id(const void* ids, int wide, int64_t i) {
   return wide ? static_cast<const int64_t*>(ids)[i] : (int64_t)static_cast<const int32_t*>(ids)[i];
 }
 
-// ---- reductions over the block ------------------------------------------------------------------------------
-template <typename V, typename Op>
-__device__ __forceinline__ V block_reduce(V v, Op op, V* tmp) {
+// ---- 16 bytes of logits ----------------------------------------------------------------------------------------
+typedef u32x4_t u32x4_any __attribute__((aligned(2)));  // at any element's address
+template <typename T>
+constexpr int kPer = 16 / (int)sizeof(T);
+template <typename T>
+__device__ __forceinline__ float elem(u32x4_t v, int i) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(v[i]);
+  else if constexpr (__is_same(T, f16_t)) return (float)__builtin_bit_cast(f16x8, v)[i];
+  else return __uint_as_float(i & 1 ? v[i / 2] & 0xFFFF0000u : v[i / 2] << 16);
+}
+template <typename T>
+__device__ __forceinline__ unsigned neg_inf_bits() {
+  return sizeof(T) == 4 ? 0xFF800000u : __is_same(T, f16_t) ? 0xFC00FC00u : 0xFF80FF80u;
+}
+template <typename T>
+__device__ __forceinline__ void drop(u32x4_t& v, int i, bool yes) {  // element i becomes -inf
+  if constexpr (sizeof(T) == 4) {
+    v[i] = yes ? neg_inf_bits<T>() : v[i];
+  } else {
+    const unsigned keep = i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+    v[i / 2] = yes ? (v[i / 2] & keep) | (neg_inf_bits<T>() & ~keep) : v[i / 2];
+  }
+}
+
+// ---- a group of NT threads: one wave of a 256-thread workgroup (NT 64), or a whole workgroup ---------------------
+template <int NT>
+__device__ __forceinline__ int group_tid() { return NT == 64 ? threadIdx.x % 64 : threadIdx.x; }
+template <int NT>
+constexpr int kBlock = NT == 64 ? 256 : NT;   // threads of a workgroup
+template <int NT>
+constexpr int kWaves = NT == 1024 ? 8 : 4;     // per SIMD, at least: two workgroups a CU
+template <int NT>
+constexpr int kGroups = NT == 64 ? 4 : 1;  // groups of a workgroup
+template <int NT>
+__device__ __forceinline__ int64_t group_index() {
+  const int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  return NT == 64 ? b * 4 + threadIdx.x / 64 : b;
+}
+template <int NT>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (NT == 64) {  // LDS operations of one wave run in order: only the compiler has to keep theirs
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    __syncthreads();
+  }
+}
+
+// wave reductions without LDS: rotations inside the rows of 16 lanes, then the row swaps of common.h
+template <int N>
+__device__ __forceinline__ float row_ror(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float wave64_sum(float v) {
+  v += row_ror<8>(v);
+  v += row_ror<4>(v);
+  v += row_ror<2>(v);
+  v += row_ror<1>(v);
+  return rows16_sum(v);
+}
+__device__ __forceinline__ float wave64_max(float v) {
+  v = fmaxf(v, row_ror<8>(v));
+  v = fmaxf(v, row_ror<4>(v));
+  v = fmaxf(v, row_ror<2>(v));
+  v = fmaxf(v, row_ror<1>(v));
+  return rows16_max(v);
+}
+__device__ __forceinline__ double wave64_sum(double v) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
-  __syncthreads();  // (tmp may still be read from the reduction before)
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ uint64_t wave64_max(uint64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint64_t w = __shfl_xor(v, o, 64);
+    v = v > w ? v : w;
+  }
+  return v;
+}
+template <int NT, typename V>
+__device__ __forceinline__ V group_sum(V v, V* tmp) {  // tmp: NT / 64 values, free when the call begins
+  v = wave64_sum(v);
+  if constexpr (NT == 64) return v;
   if (threadIdx.x % 64 == 0) tmp[threadIdx.x / 64] = v;
   __syncthreads();
   v = tmp[0];
-  for (int w = 1; w < kThreads / 64; ++w) v = op(v, tmp[w]);
+#pragma unroll
+  for (int w = 1; w < NT / 64; ++w) v += tmp[w];
   return v;
 }
-struct Add {
-  template <typename V>
-  __device__ V operator()(V a, V b) const { return a + b; }
+
+// ---- a chunk of a row in the registers of a group ----------------------------------------------------------------
+// The places are NV vectors of 16 bytes a thread, vector v of thread t being number v * NT + t of the chunk's, and, behind
+// the last whole vector, one single value each of the first threads.  Rows of odd length put the vectors at any element's
+// address.
+template <typename T, int NT, int NV>
+struct Tile {
+  u32x4_t v[NV];
+  float single;     // -inf in the threads that have none
+  int nvec, n, nv;
+
+  // column (within the chunk) of the thread's vector v / single value
+  __device__ __forceinline__ int vec_col(int vi) const { return (vi * NT + group_tid<NT>()) * kPer<T>; }
+  __device__ __forceinline__ int single_col() const { return nvec * kPer<T> + group_tid<NT>(); }
+  __device__ __forceinline__ bool has_single() const { return group_tid<NT>() < n - nvec * kPer<T>; }
+  __device__ __forceinline__ bool has_vec(int vi) const { return vi * NT + group_tid<NT>() < nvec; }
+
+  __device__ __forceinline__ void load(const T* x, int count) {
+    n = count;
+    nvec = n / kPer<T>;
+    nv = (nvec + NT - 1) / NT;
+    const u32x4_any* p = reinterpret_cast<const u32x4_any*>(x) + group_tid<NT>();
+#pragma unroll
+    for (int vi = 0; vi < NV; ++vi)
+      if (vi < nv) {
+        const unsigned none = neg_inf_bits<T>();
+        v[vi] = u32x4_t{none, none, none, none};
+        if (has_vec(vi)) v[vi] = p[vi * NT];
+      }
+    single = -kInf;
+    if (has_single()) single = (float)x[single_col()];
+  }
+  // what the mask (of the chunk's first place on) leaves out becomes -inf
+  __device__ __forceinline__ void apply_mask(const uint8_t* mask) {
+    typedef unsigned u32_any __attribute__((aligned(1)));
+#pragma unroll
+    for (int vi = 0; vi < NV; ++vi)
+      if (vi < nv && has_vec(vi)) {
+        const u32_any* p = reinterpret_cast<const u32_any*>(mask + vec_col(vi));
+        const unsigned lo = p[0], hi = kPer<T> == 8 ? (unsigned)p[kPer<T> / 8] : 0u;
+#pragma unroll
+        for (int i = 0; i < kPer<T>; ++i) drop<T>(v[vi], i, ((i < 4 ? lo : hi) >> (i % 4 * 8) & 0xFF) == 0);
+      }
+    if (has_single() && !mask[single_col()]) single = -kInf;
+  }
+  // keeps the compiler from holding the unpacked values of one pass over the tile for the next
+  __device__ __forceinline__ void pack() {
+#pragma unroll
+    for (int vi = 0; vi < NV; ++vi) asm volatile("" : "+v"(v[vi]));
+  }
+  __device__ __forceinline__ float max() const {  // (passes over NaN)
+    float m = single;
+#pragma unroll
+    for (int vi = 0; vi < NV; ++vi)
+      if (vi < nv) {
+#pragma unroll
+        for (int i = 0; i < kPer<T>; ++i) m = fmaxf(m, elem<T>(v[vi], i));
+      }
+    return m;
+  }
 };
-struct Max {
-  __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
-  __device__ uint64_t operator()(uint64_t a, uint64_t b) const { return a > b ? a : b; }
-};
-union Tmp {
-  float f[kThreads / 64];
-  double d[kThreads / 64];
-  uint64_t u[kThreads / 64];
+
+// e_j = 2^((x_j - m) c), m the largest logit, c = scale * log2(e): the difference is taken first, so that e of the largest
+// is exactly 1 (one fused x c - m c would save an operation; measured: no faster).
+struct Sums {
+  float s = 0.f, t = 0.f;  // sum e, sum e * log2 e
+  __device__ __forceinline__ void add(float d) {
+    const float e = __builtin_amdgcn_exp2f(d);
+    s += e;
+    t += e * fmaxf(d, -200.f);  // 2^-200 is 0 in fp32: a place of probability zero adds 0, not 0 * inf
+  }
 };
 
 // log p of one place, given its logit: -inf where the row holds nothing there
@@ -83,68 +223,301 @@ __device__ __forceinline__ float logp_at(float x, float m, float log_s, float sc
   return x == -kInf && log_s == log_s ? -kInf : (x - m) * scale - log_s;
 }
 
+// ---- the top alternatives -------------------------------------------------------------------------------------
+// A lower bound of the row's top-th largest logit: of the maxima of (at least top) disjoint parts of the row, the top-th
+// largest - that many places reach it.  It is looked for bit by bit in the sort key's upper half by counting over the
+// wave's lanes; the places at or above it go to a list in LDS as keys, and each key's rank is the number of larger ones.
+// 49408 normal logits, 256 parts, top 20: about 21 keys.  A list that overflows (crowded equal values) or a row with
+// NaN (which the maxima pass over) is worked off one alternative at a time instead.
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+__device__ __forceinline__ float bound_of(uint32_t prefix) {
+  return prefix < 0x00800000u ? -3.402823466e38f : key_value(prefix);  // (-inf is no alternative)
+}
+template <typename Count>
+__device__ __forceinline__ float bound_by_count(int top, Count count) {
+  uint32_t prefix = 0;
+  for (int bit = 31; bit >= 16; --bit)
+    if (count(key_value(prefix | 1u << bit)) >= top) prefix |= 1u << bit;
+  return bound_of(prefix);
+}
+constexpr int kParts = 256;  // maxima of a workgroup's parts
+template <int NT>
+constexpr int kListCap = NT == 64 ? 256 : 1024;
+
 // ---- token_logprobs -----------------------------------------------------------------------------------------
 struct ScoreArgs {
   Rows r;
+  Split sp;
   const void* targets;
   int wide_ids, n_targets, top;
   float *logprobs, *lse, *entropy, *top_logprobs, *stats;
   int64_t* top_indices;
+  float* part_sums;      // [rows, parts, 4]: m, S, sum e * log2 e of a chunk, relative to its own m
+  uint64_t* part_keys;   // [rows, parts, top]: its alternatives, best first, 0 = none
 };
 
+struct RowStats {
+  float m, log_s, h, inv_s;
+};
+// from the sums S, sum e * d (log2) relative to m
+__device__ __forceinline__ RowStats row_stats(float m, float s, float t) {
+  if (s == 0.f) return {m, -kInf, 0.f, 0.f};
+  const float log_s = logf(s);
+  return {m, log_s, log_s - t / s * kLn2, 1.f / s};
+}
+__device__ __forceinline__ void write_row(const ScoreArgs& a, int64_t row, const RowStats& st) {
+  if (a.lse) a.lse[row] = st.log_s == -kInf ? -kInf : st.m * a.r.scale + st.log_s;
+  if (a.entropy) a.entropy[row] = st.h;
+  if (a.stats) {
+    a.stats[row * 4 + 0] = st.m;
+    a.stats[row * 4 + 1] = st.log_s;
+    a.stats[row * 4 + 2] = st.h;
+    a.stats[row * 4 + 3] = st.inv_s;
+  }
+}
 template <typename T>
-__global__ __launch_bounds__(kThreads) void score_kernel(ScoreArgs a) {
-  __shared__ Tmp tmp;
-  const int64_t row = blockIdx.x;
+__device__ __forceinline__ void write_given(const ScoreArgs& a, int64_t row, const RowStats& st, int t, int threads) {
   const T* x = static_cast<const T*>(a.r.x) + row * a.r.stride;
   const uint8_t* mask = a.r.mask ? a.r.mask + row * a.r.mask_stride : nullptr;
-  const float c = a.r.scale * kLog2e;
-  float m = -kInf;
-  for (int64_t j = threadIdx.x; j < a.r.vocab; j += kThreads) m = fmaxf(m, logit(x, mask, j));
-  m = block_reduce(m, Max{}, tmp.f);
-  if (m == -kInf) m = 0.f;  // nothing allowed (the sum is 0), or nothing but NaN (the sum is NaN)
-  float s = 0.f, t = 0.f;
-  for (int64_t j = threadIdx.x; j < a.r.vocab; j += kThreads) {
-    const float d = (logit(x, mask, j) - m) * c, e = __builtin_amdgcn_exp2f(d);
-    s += e;
-    t += e * fmaxf(d, -200.f);  // 2^-200 is 0 in fp32: a place of probability zero adds 0, not 0 * inf
+  for (int i = t; i < a.n_targets; i += threads) {
+    const int64_t j = load_id(a.targets, a.wide_ids, row * a.n_targets + i);
+    float v = 0.f;
+    if (j >= a.r.vocab) v = __builtin_nanf("");
+    else if (j >= 0) v = logp_at(mask && !mask[j] ? -kInf : (float)x[j], st.m, st.log_s, a.r.scale);
+    a.logprobs[row * a.n_targets + i] = v;
   }
-  s = block_reduce(s, Add{}, tmp.f);
-  t = block_reduce(t, Add{}, tmp.f);
-  const bool empty = s == 0.f;
-  const float log_s = empty ? -kInf : logf(s);
-  const float h = empty ? 0.f : log_s - t * kLn2 / s;
-  if (threadIdx.x == 0) {
-    if (a.lse) a.lse[row] = empty ? -kInf : m * a.r.scale + log_s;
-    if (a.entropy) a.entropy[row] = h;
-    if (a.stats) {
-      a.stats[row * 4 + 0] = m;
-      a.stats[row * 4 + 1] = log_s;
-      a.stats[row * 4 + 2] = h;
-      a.stats[row * 4 + 3] = 0.f;
+}
+__device__ __forceinline__ void write_top(const ScoreArgs& a, int64_t row, const RowStats& st, int rank, uint64_t key) {
+  const bool some = (uint32_t)(key >> 32) > kKeyNegInf;
+  const float x = (uint32_t)(key >> 32) == kKeyNan ? __builtin_nanf("") : key_value((uint32_t)(key >> 32));
+  a.top_indices[row * a.top + rank] = some ? (int64_t)(0xFFFFFFFFu - (uint32_t)key) : -1;
+  a.top_logprobs[row * a.top + rank] = some ? (x - st.m) * a.r.scale - st.log_s : -kInf;
+}
+
+template <typename T, int NT, int NV, bool MASK>
+__global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs a) {
+  constexpr int G = kGroups<NT>, E = kPer<T>, CAP = kListCap<NT>;
+  __shared__ __attribute__((aligned(16))) float part_max[NT == 64 ? 1 : kParts];
+  __shared__ float tmp_s[NT / 64], tmp_t[NT / 64];
+  __shared__ uint64_t tmp_k[NT / 64];
+  __shared__ uint64_t list[G][CAP];
+  __shared__ int list_n[G];
+  const int64_t index = group_index<NT>();
+  if (index >= a.r.rows * a.sp.parts) return;
+  const int64_t row = index / a.sp.parts;
+  const int part = (int)(index - row * a.sp.parts);
+  const int g = NT == 64 ? threadIdx.x / 64 : 0, t = group_tid<NT>();
+  const int64_t first = part * a.sp.chunk;
+  const int64_t left = a.r.vocab - first;
+  const T* x = static_cast<const T*>(a.r.x) + row * a.r.stride + first;
+  Tile<T, NT, NV> tile;
+  tile.load(x, (int)(left < a.sp.chunk ? left : a.sp.chunk));
+  if constexpr (MASK) tile.apply_mask(a.r.mask + row * a.r.mask_stride + first);
+  if (t == 0) list_n[g] = 0;
+
+  // the largest logit, and a bound for the alternatives
+  float mine = tile.max(), m, bound = kInf;
+  if constexpr (NT == 64) {
+    m = wave64_max(mine);
+    if (a.top) {
+      // parts: the lanes' own places where enough of them have any; else each place for itself
+      if (a.top <= 32 && tile.nvec >= 2 * a.top) {
+        bound = bound_by_count(a.top, [&](float v) { return __popcll(__ballot(mine >= v)); });
+      } else {
+        bound = bound_by_count(a.top, [&](float v) {
+          int n = __popcll(__ballot(tile.single >= v));
+#pragma unroll
+          for (int vi = 0; vi < NV; ++vi)
+            if (vi < tile.nv) {
+#pragma unroll
+              for (int i = 0; i < E; ++i) n += __popcll(__ballot(elem<T>(tile.v[vi], i) >= v));
+            }
+          return n;
+        });
+      }
+    }
+  } else {
+    constexpr int W = NT / kParts;  // threads of a part
+    float p = mine;
+    if constexpr (W >= 2) p = fmaxf(p, __shfl_xor(p, 1, 64));
+    if constexpr (W >= 4) p = fmaxf(p, __shfl_xor(p, 2, 64));
+    if (t % W == 0) part_max[t / W] = p;
+    __syncthreads();
+    const float4 q = *reinterpret_cast<const float4*>(&part_max[t % 64 * 4]);
+    m = wave64_max(fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)));
+    if (a.top)
+      bound = bound_by_count(a.top, [&](float v) {
+        return __popcll(__ballot(q.x >= v)) + __popcll(__ballot(q.y >= v)) + __popcll(__ballot(q.z >= v)) +
+               __popcll(__ballot(q.w >= v));
+      });
+  }
+
+  // sums, and the places at or above the bound
+  tile.pack();
+  if (m == -kInf) m = 0.f;  // nothing allowed (the sum is 0), or nothing but NaN (the sum is NaN)
+  const float c = a.r.scale * kLog2e;
+  Sums sums;
+  const auto keep = [&](float v, int col) {
+    const int at = atomicAdd(&list_n[g], 1);
+    if (at < CAP) list[g][at] = place_key(v, (uint32_t)(first + col));
+  };
+  if constexpr (NT == 64) group_sync<NT>();  // (list_n is 0)
+#pragma unroll
+  for (int vi = 0; vi < NV; ++vi)
+    if (vi < tile.nv) {
+      float best = -kInf;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const float v = elem<T>(tile.v[vi], i);
+        best = fmaxf(best, v);
+        sums.add((v - m) * c);
+      }
+      if (best >= bound) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const float v = elem<T>(tile.v[vi], i);
+          if (v >= bound) keep(v, tile.vec_col(vi) + i);
+        }
+      }
+    }
+  sums.add((tile.single - m) * c);
+  if (tile.single >= bound) keep(tile.single, tile.single_col());
+  sums.s = wave64_sum(sums.s);
+  sums.t = wave64_sum(sums.t);
+  if constexpr (NT == 64) {
+    group_sync<NT>();
+  } else {
+    if (t % 64 == 0) {
+      tmp_s[t / 64] = sums.s;
+      tmp_t[t / 64] = sums.t;
+    }
+    __syncthreads();
+    sums.s = tmp_s[0];
+    sums.t = tmp_t[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) {
+      sums.s += tmp_s[w];
+      sums.t += tmp_t[w];
     }
   }
-  for (int i = threadIdx.x; i < a.n_targets; i += kThreads) {
-    const int64_t j = load_id(a.targets, a.wide_ids, row * a.n_targets + i);
-    a.logprobs[row * a.n_targets + i] = j < 0               ? 0.f
-                                        : j >= a.r.vocab ? __builtin_nanf("")
-                                                            : logp_at(logit(x, mask, j), m, log_s, a.r.scale);
+
+  RowStats st;
+  const bool whole = a.sp.parts == 1;
+  if (whole) {
+    st = row_stats(m, sums.s, sums.t);
+    if (t == 0) write_row(a, row, st);
+    write_given<T>(a, row, st, t, NT);
+  } else if (t == 0) {
+    float* p = a.part_sums + index * 4;
+    p[0] = m;
+    p[1] = sums.s;
+    p[2] = sums.t;
   }
+  if (a.top == 0) return;
+  const auto put = [&](int rank, uint64_t key) {
+    if (whole) write_top(a, row, st, rank, key);
+    else a.part_keys[index * a.top + rank] = key;
+  };
+  const int n = list_n[g];
+  if (n <= CAP && sums.s == sums.s) {
+    constexpr int R = NT == 64 ? 2 : 8;  // lanes that count for one key
+    for (int i = t / R; i < n; i += NT / R) {
+      const uint64_t key = list[g][i];
+      int rank = 0;
+#pragma unroll 8
+      for (int k = t % R; k < n; k += R) rank += list[g][k] > key;
+#pragma unroll
+      for (int o = 1; o < R; o *= 2) rank += __shfl_xor(rank, o, 64);
+      if (t % R == 0 && rank < a.top) put(rank, key);
+    }
+    for (int i = n + t; i < a.top; i += NT) put(i, 0);
+    return;
+  }
+  // (from memory again: the tile's registers are not held for the rare case)
   uint64_t last = ~0ull;
+  const uint8_t* mask = MASK ? a.r.mask + row * a.r.mask_stride + first : nullptr;
   for (int i = 0; i < a.top; ++i) {
     uint64_t best = 0;
-    for (int64_t j = threadIdx.x; j < a.r.vocab; j += kThreads) {
-      const uint64_t k = place_key(logit(x, mask, j), (uint32_t)j);
-      if (k < last && k > best) best = k;
+    for (int j = t; j < tile.n; j += NT) {
+      const uint64_t key = place_key(MASK && !mask[j] ? -kInf : (float)x[j], (uint32_t)(first + j));
+      if (key < last && key > best && (uint32_t)(key >> 32) > kKeyNegInf) best = key;
     }
-    last = block_reduce(best, Max{}, tmp.u);
-    if (threadIdx.x == 0) {
-      const bool some = (uint32_t)(last >> 32) > kKeyNegInf;
-      const int64_t j = some ? 0xFFFFFFFFu - (uint32_t)last : 0;
-      a.top_indices[row * a.top + i] = some ? j : -1;
-      a.top_logprobs[row * a.top + i] = some ? logp_at((float)x[j], m, log_s, a.r.scale) : -kInf;
+    best = wave64_max(best);
+    if constexpr (NT != 64) {
+      if (t % 64 == 0) tmp_k[t / 64] = best;
+      __syncthreads();
+      for (int w = 0; w < NT / 64; ++w) best = tmp_k[w] > best ? tmp_k[w] : best;
+      __syncthreads();
     }
+    if (t == 0) put(i, best);
+    last = best;  // (0 when nothing is left: nothing is below it)
   }
+}
+
+// The chunks of a row joined: sums brought to the largest m, in the chunks' order, and the chunks' lists merged - the rank
+// of a key is its place in its own list plus, for each other list, how many keys of that are larger (a binary search).
+constexpr int kJoinCap = 4096;  // keys that are looked at in LDS (32 KB); more stay in memory
+template <typename T>
+__global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
+  __shared__ uint64_t list[kJoinCap];
+  const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  if (row >= a.r.rows) return;
+  const int t = threadIdx.x, parts = a.sp.parts, top = a.top;
+  const float* p = a.part_sums + row * parts * 4;
+  const float c = a.r.scale * kLog2e;
+  // every wave for itself: no exchange
+  float m = -kInf, s = 0.f, u = 0.f;
+  for (int i = t % 64; i < parts; i += 64)
+    if (p[i * 4 + 1] != 0.f) m = fmaxf(m, p[i * 4]);
+  m = wave64_max(m);
+  if (m == -kInf) m = 0.f;
+  for (int i = t % 64; i < parts; i += 64) {
+    const float si = p[i * 4 + 1], ui = p[i * 4 + 2];
+    if (si == 0.f) continue;
+    const float d = (p[i * 4] - m) * c, f = __builtin_amdgcn_exp2f(d);
+    s += f * si;
+    u += f * (ui + si * fmaxf(d, -200.f));
+  }
+  s = wave64_sum(s);
+  u = wave64_sum(u);
+  const RowStats st = row_stats(m, s, u);
+  if (t == 0) write_row(a, row, st);
+  write_given<T>(a, row, st, t, kThreads);
+  if (top == 0) return;
+
+  const int64_t total = (int64_t)parts * top;
+  const uint64_t* all = a.part_keys + row * total;
+  int some = 0;  // alternatives of the row that this thread has seen: the rest of the answer is filled up
+  const auto merge = [&](const uint64_t* keys) {
+    for (int64_t i = t; i < total; i += kThreads) {
+      const uint64_t key = keys[i];
+      if (key == 0) continue;
+      ++some;
+      const int own = (int)(i / top);
+      int64_t rank = i - (int64_t)own * top;
+#pragma unroll 4
+      for (int p = 0; p < parts; ++p) {
+        if (p == own) continue;
+        const uint64_t* other = keys + (int64_t)p * top;
+        int lo = 0;  // keys of the other list before `lo` are larger
+        for (int step = kMaxTop; step > 0; step /= 2)
+          if (lo + step <= top && other[lo + step - 1] > key) lo += step;
+        rank += lo;
+      }
+      if (rank < top) write_top(a, row, st, (int)rank, key);
+    }
+  };
+  if (total <= kJoinCap) {
+    for (int i = t; i < (int)total; i += kThreads) list[i] = all[i];
+    __syncthreads();
+    merge(list);
+  } else {
+    merge(all);
+  }
+  __shared__ float tmp[kThreads / 64];
+  const float found = group_sum<kThreads>((float)some, tmp);
+  for (int i = t; i < top; i += kThreads)
+    if (i >= found) write_top(a, row, st, i, 0);
 }
 
 // ---- the teacher's list of one row ----------------------------------------------------------------------------
@@ -153,122 +526,290 @@ struct TeacherArgs {
   const float* v;
   int wide_ids, n, tail;
 };
-struct Teacher {       // (in LDS)
-  int id[kMaxList];    // -1: absent
-  float v[kMaxList], q[kMaxList];
-  float q_sum, q_rest, log_norm;  // sum of q; the bucket's probability; log q = v - log_norm
-  bool some;                      // there is an entry at all
+// one entry: its place (-1: absent, or no place of the vocabulary) and its log probability (-inf: absent; NaN: loud)
+__device__ __forceinline__ float teacher_entry(const TeacherArgs& a, int64_t row, int64_t vocab, int i, int& id) {
+  const int64_t j = load_id(a.ids, a.wide_ids, row * a.n + i);
+  float v = a.v[row * a.n + i];
+  if (j < 0) v = -kInf;
+  if (j >= vocab && v != -kInf) v = __builtin_nanf("");
+  id = v == -kInf || j >= vocab ? -1 : (int)j;
+  return v;
+}
+// q = e^(v - log_norm): the softmax of the row's entries, or (tail) e^v as they are and a bucket for what is left of 1,
+// a difference from 1 that is taken in 64 bits
+struct Teacher {
+  float log_norm, q_sum, q_rest;
+  bool some;  // there is an entry at all
 };
-
-// q of a row: the softmax of its entries, or (tail) e^v as they are and a bucket for what is left of 1.  The bucket is a
-// difference from 1, taken in 64 bits.  An id that the vocabulary does not have makes the row NaN.
-__device__ __forceinline__ void teacher_row(const TeacherArgs& a, int64_t row, int64_t vocab, Teacher& s, Tmp& tmp) {
+template <int CAP>
+struct TeacherList {  // in LDS
+  int id[CAP];
+  float v[CAP];
+  Teacher t;
+};
+// e^v in 64 bits for what stands in a list: v = n log 2 + r, the series of e^r (|r| <= 0.35: the 12th term is below 1e-14).
+// (The library's exp would take the workgroup of 1024 past 64 registers a thread, and so to one a CU.)
+__device__ __forceinline__ double exp64(double v) {
+  const double n = __builtin_rint(v * 1.4426950408889634), r = __builtin_fma(n, -0.69314718055994531, v);
+  double p = 1.0;
+#pragma unroll
+  for (int k = 11; k > 0; --k) p = __builtin_fma(p * (1.0 / k), r, 1.0);
+  return v < -200.0 ? 0.0 : __builtin_ldexp(p, (int)n);
+}
+// by one wave (every lane of it), for the group
+template <int CAP>
+__device__ __forceinline__ void teacher_row(const TeacherArgs& a, int64_t row, int64_t vocab, TeacherList<CAP>& s) {
+  const int lane = threadIdx.x % 64;
   float best = -kInf, some = 0.f;
-  for (int i = threadIdx.x; i < a.n; i += kThreads) {
-    const int64_t j = load_id(a.ids, a.wide_ids, row * a.n + i);
-    float v = a.v[row * a.n + i];
-    if (j < 0) v = -kInf;
-    if (j >= vocab && v != -kInf) v = __builtin_nanf("");
-    s.id[i] = v == -kInf || j >= vocab ? -1 : (int)j;
+  for (int i = lane; i < a.n; i += 64) {
+    int id;
+    const float v = teacher_entry(a, row, vocab, i, id);
+    s.id[i] = id;
     s.v[i] = v;
     best = fmaxf(best, v);
     if (v != -kInf) some = 1.f;
   }
-  best = block_reduce(best, Max{}, tmp.f);
-  some = block_reduce(some, Max{}, tmp.f);
+  best = wave64_max(best);
+  some = wave64_max(some);
   if (a.tail || best == -kInf) best = 0.f;  // (no entry: every q is 0)
+  group_sync<64>();
   double sum = 0;
-  for (int i = threadIdx.x; i < a.n; i += kThreads) sum += exp((double)(s.v[i] - best));
-  sum = block_reduce(sum, Add{}, tmp.d);
-  const float log_norm = a.tail || sum == 0 ? best : best + (float)log(sum);
+  for (int i = lane; i < a.n; i += 64) sum += exp64((double)s.v[i] - best);
+  sum = wave64_sum(sum);
+  const float log_norm = a.tail || sum == 0 ? best : best + logf((float)sum);
   float q_sum = 0.f;
-  for (int i = threadIdx.x; i < a.n; i += kThreads) {
-    const float q = a.tail || sum == 0 ? expf(s.v[i]) : expf(s.v[i] - best) / (float)sum;
-    s.q[i] = q;
-    q_sum += q;
-  }
-  q_sum = block_reduce(q_sum, Add{}, tmp.f);
-  if (threadIdx.x == 0) {
-    s.q_sum = q_sum;
-    s.q_rest = a.tail ? (float)(sum > 1 ? 0 : 1 - sum) : 0.f;
-    s.log_norm = log_norm;
-    s.some = some != 0.f;
-  }
-  __syncthreads();
-}
-__device__ __forceinline__ bool listed(const Teacher& s, int n, int64_t j) {
-  for (int i = 0; i < n; ++i)
-    if (s.id[i] == j) return true;
-  return false;
+  for (int i = lane; i < a.n; i += 64) q_sum += expf(s.v[i] - log_norm);
+  q_sum = wave64_sum(q_sum);
+  if (lane == 0) s.t = {log_norm, q_sum, a.tail ? (float)(sum > 1 ? 0 : 1 - sum) : 0.f, some != 0.f};
 }
 
+// ---- distill_top_logits -----------------------------------------------------------------------------------------
 struct DistillArgs {
   Rows r;
+  Split sp;
   TeacherArgs t;
   float *loss, *stats;
+  float* part_sums;  // [rows, parts, 2]: m, S of a chunk (tail: of its places outside the list)
 };
+// What the backward pass needs of a row: m, 1 / S (0: the student has nothing); the same outside the list; the student's
+// probability there; the teacher's log_norm, q_sum (-1: no entry) and bucket
+constexpr int kStats = 8;
+__device__ __forceinline__ void write_no_teacher(const DistillArgs& a, int64_t row) {
+  a.loss[row] = 0.f;
+  a.stats[row * kStats + 6] = -1.f;
+}
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_kernel(DistillArgs a) {
-  __shared__ Tmp tmp;
-  __shared__ Teacher te;
-  const int64_t row = blockIdx.x;
+// log s to about 2^-25 whatever its size, for the few places whose log p and log q are nearly equal
+__device__ __forceinline__ double log64(float s) {
+  const int n = __builtin_amdgcn_frexp_expf(s);
+  return (double)logf(__builtin_ldexpf(s, -n)) + n * 0.69314718055994531;
+}
+// The end of a row, by one group: `m` and `s` are the row's largest logit and sum (tail: of the places outside the list;
+// the listed ones are added here, each place once).
+template <typename T, int NT, int CAP>
+__device__ __forceinline__ void finish_distill(const DistillArgs& a, int64_t row, const TeacherList<CAP>& te, bool distinct,
+                                               float m, float s, float* tmp) {
   const T* x = static_cast<const T*>(a.r.x) + row * a.r.stride;
-  const float c = a.r.scale * kLog2e;
-  teacher_row(a.t, row, a.r.vocab, te, tmp);
-  if (!te.some) {  // no teacher: no loss (the backward pass reads the list again, and no statistics)
-    if (threadIdx.x == 0) a.loss[row] = 0.f;
+  const int t = group_tid<NT>(), n = a.t.n;
+  const float scale = a.r.scale, mo = m, so = s;
+  float p_o = 1.f;
+  if (a.t.tail) {
+    float peak = so == 0.f ? -kInf : mo;
+    // (few values: every wave looks at all of them)
+    for (int i = t % 64; i < n; i += 64)
+      if (te.id[i] >= 0) peak = fmaxf(peak, (float)x[te.id[i]]);
+    peak = wave64_max(peak);
+    m = peak == -kInf ? 0.f : peak;
+    s = 0.f;
+    for (int i = t % 64; i < n; i += 64) {
+      bool first = te.id[i] >= 0;
+      if (!distinct)
+        for (int k = 0; k < i; ++k) first = first && te.id[k] != te.id[i];
+      if (first) s += __builtin_amdgcn_exp2f(((float)x[te.id[i]] - m) * (scale * kLog2e));
+    }
+    s = wave64_sum(s);
+    p_o = so == 0.f ? 0.f : so * __builtin_amdgcn_exp2f((mo - m) * (scale * kLog2e));
+    s += p_o;
+    p_o /= s;
+  }
+  const double log_s = log64(s);
+  float loss = 0.f;
+  for (int i = t; i < n; i += NT) {
+    const float v = te.v[i], q = expf(v - te.t.log_norm);
+    if (q == 0.f) continue;
+    const float y = te.id[i] < 0 ? v : (float)x[te.id[i]];  // (an id that the vocabulary does not have: v is NaN)
+    const float lost = y == -kInf && s == s ? kInf : (float)((double)v - te.t.log_norm - ((double)y - m) * scale + log_s);
+    loss += q * lost;
+  }
+  loss = group_sum<NT>(loss, tmp);
+  if (t == 0) {
+    const float rest = !a.t.tail || so == 0.f ? 0.f : te.t.q_rest;
+    if (rest != 0.f) loss += rest * (float)(log64(rest) - ((double)mo - m) * scale - log64(so) + log_s);
+    a.loss[row] = loss;
+    float* st = a.stats + row * kStats;
+    st[0] = m;
+    st[1] = s == 0.f ? 0.f : 1.f / s;
+    st[2] = mo;
+    st[3] = so == 0.f ? 0.f : 1.f / so;
+    st[4] = p_o;
+    st[5] = te.t.log_norm;
+    st[6] = te.t.q_sum;
+    st[7] = rest;
+  }
+}
+
+// Places of a chunk by the bits of a map in LDS: vectors first (a vector's bits are a byte, or half of one), then the
+// single places.
+template <typename T, int NT, int NV, bool TAIL, int LIST>
+__global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(DistillArgs a) {
+  constexpr int G = kGroups<NT>, E = kPer<T>, WORDS = TAIL ? NT * NV * E / 32 + 1 : 1;
+  __shared__ TeacherList<LIST> te[G];
+  __shared__ unsigned map[G][WORDS];
+  __shared__ int twice[G];
+  __shared__ float tmp_m[NT / 64], tmp_s[NT / 64], tmp_l[NT / 64];
+  const int64_t index = group_index<NT>();
+  if (index >= a.r.rows * a.sp.parts) return;
+  const int64_t row = index / a.sp.parts;
+  const int part = (int)(index - row * a.sp.parts);
+  const int g = NT == 64 ? threadIdx.x / 64 : 0, t = group_tid<NT>();
+  const int64_t first = part * a.sp.chunk;
+  const int64_t left = a.r.vocab - first;
+  const T* x = static_cast<const T*>(a.r.x) + row * a.r.stride + first;
+  const bool whole = a.sp.parts == 1;
+  Tile<T, NT, NV> tile;
+  tile.load(x, (int)(left < a.sp.chunk ? left : a.sp.chunk));
+  if (t == 0) twice[g] = 0;
+  if constexpr (TAIL) {
+    for (int i = t; i < WORDS; i += NT) map[g][i] = 0;
+    group_sync<NT>();
+  }
+  if (t < 64 && (TAIL || whole)) {
+    teacher_row(a.t, row, a.r.vocab, te[g]);
+    if constexpr (TAIL) {
+      for (int i = t; i < a.t.n; i += 64) {
+        const int64_t col = te[g].id[i] - first;
+        if (te[g].id[i] < 0 || col < 0 || col >= tile.n) continue;
+        const int nv = tile.nvec * E, bit = col < nv ? (int)col : NT * NV * E + (int)col - nv;
+        if (atomicOr(&map[g][bit / 32], 1u << bit % 32) >> bit % 32 & 1) twice[g] = 1;
+      }
+    }
+  }
+  if constexpr (TAIL) {  // what the list holds is left out
+    group_sync<NT>();
+#pragma unroll
+    for (int vi = 0; vi < NV; ++vi)
+      if (vi < tile.nv) {
+        const int q = vi * NT + t;
+        const unsigned bits = map[g][q * E / 32] >> q * E % 32 & ((1u << E) - 1);
+        if (bits) {
+#pragma unroll
+          for (int i = 0; i < E; ++i) drop<T>(tile.v[vi], i, bits >> i & 1);
+        }
+      }
+    if (t < 32 && map[g][NT * NV * E / 32] >> t & 1) tile.single = -kInf;
+  }
+  float m = wave64_max(tile.max());
+  if constexpr (NT != 64) {
+    if (t % 64 == 0) tmp_m[t / 64] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) m = fmaxf(m, tmp_m[w]);
+  } else {
+    group_sync<NT>();
+  }
+  if ((TAIL || whole) && !te[g].t.some) {  // no teacher: no loss
+    if (t == 0 && whole) write_no_teacher(a, row);
     return;
   }
-  float m = -kInf, mo = -kInf;  // all places; the places outside the list
-  for (int64_t j = threadIdx.x; j < a.r.vocab; j += kThreads) {
-    const float v = (float)x[j];
-    m = fmaxf(m, v);
-    if (a.t.tail && !listed(te, a.t.n, j)) mo = fmaxf(mo, v);
-  }
-  m = block_reduce(m, Max{}, tmp.f);
-  mo = block_reduce(mo, Max{}, tmp.f);
   if (m == -kInf) m = 0.f;
-  if (mo == -kInf) mo = 0.f;
-  float s = 0.f, so = 0.f;
-  for (int64_t j = threadIdx.x; j < a.r.vocab; j += kThreads) {
-    const float v = (float)x[j];
-    s += __builtin_amdgcn_exp2f((v - m) * c);
-    if (a.t.tail && !listed(te, a.t.n, j)) so += __builtin_amdgcn_exp2f((v - mo) * c);
-  }
-  s = block_reduce(s, Add{}, tmp.f);
-  so = block_reduce(so, Add{}, tmp.f);
-  const float log_s = s == 0.f ? -kInf : logf(s), log_so = so == 0.f ? -kInf : logf(so);
-  float loss = 0.f;
-  for (int i = threadIdx.x; i < a.t.n; i += kThreads)
-    if (te.q[i] != 0.f) {
-      const float lp = te.id[i] < 0 ? 0.f : logp_at((float)x[te.id[i]], m, log_s, a.r.scale);
-      loss += te.q[i] * (te.v[i] - te.log_norm - lp);
+  const float c = a.r.scale * kLog2e;
+  float s = __builtin_amdgcn_exp2f((tile.single - m) * c);
+  tile.pack();
+#pragma unroll
+  for (int vi = 0; vi < NV; ++vi)
+    if (vi < tile.nv) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) s += __builtin_amdgcn_exp2f((elem<T>(tile.v[vi], i) - m) * c);
     }
-  loss = block_reduce(loss, Add{}, tmp.f);
-  if (threadIdx.x == 0) {
-    const float rest = log_so == -kInf ? 0.f : te.q_rest;
-    if (rest != 0.f) loss += rest * (logf(rest) - ((mo - m) * a.r.scale + log_so - log_s));
-    a.loss[row] = loss;
-    a.stats[row * 8 + 0] = m;
-    a.stats[row * 8 + 1] = log_s;
-    a.stats[row * 8 + 2] = mo;
-    a.stats[row * 8 + 3] = log_so;
+  s = group_sum<NT>(s, tmp_s);
+  if (whole) {
+    finish_distill<T, NT>(a, row, te[g], TAIL && !twice[g], m, s, tmp_l);
+  } else if (t == 0) {
+    a.part_sums[index * 2] = m;
+    a.part_sums[index * 2 + 1] = s;
   }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void distill_join_kernel(DistillArgs a) {
+  __shared__ TeacherList<kMaxList> te;
+  __shared__ float tmp[kThreads / 64];
+  const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  if (row >= a.r.rows) return;
+  const int t = threadIdx.x, parts = a.sp.parts;
+  if (t < 64) teacher_row(a.t, row, a.r.vocab, te);
+  __syncthreads();
+  if (!te.t.some) {
+    if (t == 0) write_no_teacher(a, row);
+    return;
+  }
+  const float* p = a.part_sums + row * parts * 2;
+  float m = -kInf, s = 0.f;
+  for (int i = t % 64; i < parts; i += 64)
+    if (p[i * 2 + 1] != 0.f) m = fmaxf(m, p[i * 2]);
+  m = wave64_max(m);
+  if (m == -kInf) m = 0.f;
+  for (int i = t % 64; i < parts; i += 64)
+    if (p[i * 2 + 1] != 0.f) s += p[i * 2 + 1] * __builtin_amdgcn_exp2f((p[i * 2] - m) * (a.r.scale * kLog2e));
+  s = wave64_sum(s);
+  finish_distill<T, kThreads>(a, row, te, false, m, s, tmp);
 }
 
 // ---- gradients --------------------------------------------------------------------------------------------------
 // Both operators' gradients are, over the whole row, p'_j * (a0 + a1 * (log p_j + H)) with p' = e^(d' - log S'), and at
 // the few listed places j (given tokens and alternatives; the teacher's list) b0 * p_j + ... plus the weights of the
-// entries that name j.  The row is written first, then the listed places again, each by the first entry that names it
-// with the weights of all of them, so that no sum depends on an order.
-template <typename T>
-__device__ __forceinline__ void fill(T* g, int64_t n, float v) {
-  for (int64_t j = threadIdx.x; j < n; j += kThreads) g[j] = to16<T>(v);
+// entries that name j.  A chunk is written whole first, then its listed places again, each by the first entry that names
+// it with the weights of all of them, so that no sum depends on an order.
+template <typename T, int NT, int NV, typename F>
+__device__ __forceinline__ void write_dense(const Tile<T, NT, NV>& tile, T* g, F value) {
+#pragma unroll
+  for (int vi = 0; vi < NV; ++vi)
+    if (vi < tile.nv && tile.has_vec(vi)) {
+      u32x4_t out;
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = __float_as_uint(value(elem<T>(tile.v[vi], i)));
+      } else {
+        typename T16<T>::vec8 o;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = to16<T>(value(elem<T>(tile.v[vi], i)));
+        out = __builtin_bit_cast(u32x4_t, o);
+      }
+      *reinterpret_cast<u32x4_any*>(g + tile.vec_col(vi)) = out;
+    }
+  if (tile.has_single()) g[tile.single_col()] = to16<T>(value(tile.single));
+}
+// the listed places of a chunk; value(x, weight)
+template <typename T, int NT, typename F>
+__device__ __forceinline__ void write_listed(const int* id, const float* w, int n, const T* x, T* g, int64_t first, int count,
+                                             F value) {
+  for (int i = group_tid<NT>(); i < n; i += NT) {
+    const int j = id[i];
+    if (j < first || j >= first + count) continue;  // (-1: no place)
+    float sum = 0.f;
+    bool before = false;
+    for (int k = 0; k < n; ++k)
+      if (id[k] == j) {
+        before = before || k < i;
+        sum += w[k];
+      }
+    if (!before) g[j - first] = to16<T>(value((float)x[j - first], sum));
+  }
 }
 
 struct ScoreGradArgs {
   Rows r;
+  Split sp;
   const void* targets;
   int wide_ids, n_targets, top;
   const int64_t* top_indices;
@@ -277,95 +818,139 @@ struct ScoreGradArgs {
   int64_t grad_stride;
 };
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void score_grad_kernel(ScoreGradArgs a) {
-  __shared__ Tmp tmp;
-  __shared__ int id[kMaxList + kMaxTop];
-  __shared__ float w[kMaxList + kMaxTop];
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(a.r.x) + row * a.r.stride;
-  const uint8_t* mask = a.r.mask ? a.r.mask + row * a.r.mask_stride : nullptr;
-  T* g = static_cast<T*>(a.grad) + row * a.grad_stride;
-  const float m = a.stats[row * 4], log_s = a.stats[row * 4 + 1], h = a.stats[row * 4 + 2];
-  if (log_s == -kInf) return fill(g, a.r.vocab, 0.f);
+template <typename T, int NT, int NV, bool MASK, int LIST>
+__global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_grad_kernel(ScoreGradArgs a) {
+  constexpr int G = kGroups<NT>;
+  __shared__ int ids[G][LIST];
+  __shared__ float ws[G][LIST];
+  __shared__ float tmp[NT / 64];
+  const int64_t index = group_index<NT>();
+  if (index >= a.r.rows * a.sp.parts) return;
+  const int64_t row = index / a.sp.parts;
+  const int64_t first = (index - row * a.sp.parts) * a.sp.chunk;
+  const int64_t left = a.r.vocab - first;
+  const T* xr = static_cast<const T*>(a.r.x) + row * a.r.stride;
+  const uint8_t* mask = MASK ? a.r.mask + row * a.r.mask_stride : nullptr;
+  T* g = static_cast<T*>(a.grad) + row * a.grad_stride + first;
+  Tile<T, NT, NV> tile;
+  tile.load(xr + first, (int)(left < a.sp.chunk ? left : a.sp.chunk));
+  if constexpr (MASK) tile.apply_mask(mask + first);
+  int* id = ids[NT == 64 ? threadIdx.x / 64 : 0];
+  float* w = ws[NT == 64 ? threadIdx.x / 64 : 0];
+  const float m = a.stats[row * 4], log_s = a.stats[row * 4 + 1], h = a.stats[row * 4 + 2], inv_s = a.stats[row * 4 + 3];
+  const float scale = a.r.scale;
   const int nt = a.g_logprobs ? a.n_targets : 0, n = nt + (a.g_top ? a.top : 0);
   float sum = 0.f;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
+  for (int i = group_tid<NT>(); i < n; i += NT) {
     const int64_t j = i < nt ? load_id(a.targets, a.wide_ids, row * a.n_targets + i) : a.top_indices[row * a.top + i - nt];
     float v = i < nt ? a.g_logprobs[row * a.n_targets + i] : a.g_top[row * a.top + i - nt];
-    if (j < 0) v = 0.f;                                              // padding
-    else if (j >= a.r.vocab) v = __builtin_nanf("");                // (its log probability is NaN)
-    else if (logit(x, mask, j) == -kInf) v = 0.f;                   // -inf whatever the logits: a constant
+    if (j < 0) v = 0.f;                                                    // padding
+    else if (j >= a.r.vocab) v = __builtin_nanf("");                      // (its log probability is NaN)
+    else if ((MASK && !mask[j]) || (float)xr[j] == -kInf) v = 0.f;        // -inf whatever the logits: a constant
     id[i] = j < 0 || j >= a.r.vocab || v == 0.f ? -1 : (int)j;
     w[i] = v;
     sum += v;
   }
-  sum = block_reduce(sum, Add{}, tmp.f);
+  sum = n ? group_sum<NT>(sum, tmp) : 0.f;  // (its barrier is the lists' too)
+  if constexpr (NT == 64) group_sync<NT>();
   const float gh = a.g_entropy ? a.g_entropy[row] : 0.f;
   const float a0 = (a.g_lse ? a.g_lse[row] : 0.f) - sum;
-  const float scale = a.r.scale;
-  const auto dense = [&](float v) {  // dH / dz_j = -p_j (log p_j + H)
-    const float lp = fmaxf((v - m) * scale - log_s, -150.f);
-    return __builtin_amdgcn_exp2f((v - m) * (scale * kLog2e) - log_s * kLog2e) * (a0 - gh * (lp + h));
+  const bool empty = log_s == -kInf;
+  // p_j (a0 - g_H (log p_j + H)) with p_j = e^d_j / S (not e^(d_j - log S): log S has lost digits to its size)
+  const float c = scale * kLog2e, b0 = a0 - gh * (h - log_s), b1 = gh * kLn2;
+  const auto dense = [&](float x) {
+    const float d = (x - m) * c;
+    return __builtin_amdgcn_exp2f(d) * inv_s * (b0 - b1 * fmaxf(d, -200.f));
   };
-  for (int64_t j = threadIdx.x; j < a.r.vocab; j += kThreads)
-    g[j] = to16<T>(mask && !mask[j] ? 0.f : dense((float)x[j]) * scale);
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    if (id[i] < 0) continue;
-    float v = 0.f;
-    bool first = true;
-    for (int k = 0; k < n; ++k)
-      if (id[k] == id[i]) {
-        first = first && k >= i;
-        v += w[k];
-      }
-    if (first) g[id[i]] = to16<T>((dense((float)x[id[i]]) + v) * scale);
+  if (empty) {
+    write_dense<T, NT, NV>(tile, g, [](float) { return 0.f; });
+    return;
   }
+  write_dense<T, NT, NV>(tile, g, [&](float x) {
+    const float v = dense(x) * scale;
+    return MASK && x == -kInf ? 0.f : v;
+  });
+  if (n == 0) return;
+  group_sync<NT>();
+  write_listed<T, NT>(id, w, n, xr + first, g, first, tile.n, [&](float x, float v) { return (dense(x) + v) * scale; });
 }
 
 struct DistillGradArgs {
   Rows r;
+  Split sp;
   TeacherArgs t;
   const float *stats, *g_loss;
   void* grad;
   int64_t grad_stride;
 };
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_grad_kernel(DistillGradArgs a) {
-  __shared__ Tmp tmp;
-  __shared__ Teacher te;
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(a.r.x) + row * a.r.stride;
-  T* g = static_cast<T*>(a.grad) + row * a.grad_stride;
-  teacher_row(a.t, row, a.r.vocab, te, tmp);
-  if (!te.some) return fill(g, a.r.vocab, 0.f);
-  const float m = a.stats[row * 8], log_s = a.stats[row * 8 + 1], mo = a.stats[row * 8 + 2], log_so = a.stats[row * 8 + 3];
-  if (log_s == -kInf) return fill(g, a.r.vocab, 0.f);
-  const float up = a.g_loss[row] * a.r.scale, c = a.r.scale * kLog2e;
-  const bool tail = a.t.tail && log_so != -kInf;
-  const float rest = tail ? te.q_rest : 0.f, q_all = te.q_sum + rest;
-  // outside the list: p_j q_all - rest e^(z_j - lse_o) = e^(z_j - lse_o) (p_o q_all - rest), p_o the student's bucket
-  const float ref = tail ? mo : m, log_ref = (tail ? log_so : log_s) * kLog2e;
-  const float p_o = tail ? expf((mo - m) * a.r.scale + log_so - log_s) : 1.f;
-  const float a0 = up * (p_o * q_all - rest);
-  for (int64_t j = threadIdx.x; j < a.r.vocab; j += kThreads)
-    g[j] = to16<T>(a0 * __builtin_amdgcn_exp2f(((float)x[j] - ref) * c - log_ref));
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.t.n; i += kThreads) {
-    if (te.id[i] < 0) continue;
-    float q = 0.f;
-    bool first = true;
-    for (int k = 0; k < a.t.n; ++k)
-      if (te.id[k] == te.id[i]) {
-        first = first && k >= i;
-        q += te.q[k];
-      }
-    const float p = __builtin_amdgcn_exp2f(((float)x[te.id[i]] - m) * c - log_s * kLog2e);
-    if (first) g[te.id[i]] = to16<T>(up * (p * q_all - q));
+template <typename T, int NT, int NV, int LIST>
+__global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_grad_kernel(DistillGradArgs a) {
+  constexpr int G = kGroups<NT>;
+  __shared__ int ids[G][LIST];
+  __shared__ float ws[G][LIST];
+  const int64_t index = group_index<NT>();
+  if (index >= a.r.rows * a.sp.parts) return;
+  const int64_t row = index / a.sp.parts;
+  const int64_t first = (index - row * a.sp.parts) * a.sp.chunk;
+  const int64_t left = a.r.vocab - first;
+  const T* x = static_cast<const T*>(a.r.x) + row * a.r.stride + first;
+  T* g = static_cast<T*>(a.grad) + row * a.grad_stride + first;
+  Tile<T, NT, NV> tile;
+  tile.load(x, (int)(left < a.sp.chunk ? left : a.sp.chunk));
+  int* id = ids[NT == 64 ? threadIdx.x / 64 : 0];
+  float* w = ws[NT == 64 ? threadIdx.x / 64 : 0];
+  const float* st = a.stats + row * kStats;
+  const float m = st[0], inv_s = st[1], mo = st[2], inv_so = st[3], p_o = st[4], log_norm = st[5], q_sum = st[6], rest = st[7];
+  if (q_sum == -1.f || inv_s == 0.f) {
+    write_dense<T, NT, NV>(tile, g, [](float) { return 0.f; });
+    return;
   }
+  for (int i = group_tid<NT>(); i < a.t.n; i += NT) {
+    int j;
+    w[i] = expf(teacher_entry(a.t, row, a.r.vocab, i, j) - log_norm);
+    id[i] = j;
+  }
+  const float up = a.g_loss[row] * a.r.scale, c = a.r.scale * kLog2e;
+  const bool tail = a.t.tail && inv_so != 0.f;
+  const float q_all = q_sum + rest;
+  // outside the list: p_j q_all - rest e^(z_j - lse_o) = e^(z_j - lse_o) (p_o q_all - rest), p_o the student's bucket
+  const float from = tail ? mo : m, a0 = tail ? up * (p_o * q_all - rest) * inv_so : up * q_all * inv_s;
+  write_dense<T, NT, NV>(tile, g, [&](float v) { return a0 * __builtin_amdgcn_exp2f((v - from) * c); });
+  group_sync<NT>();
+  write_listed<T, NT>(id, w, a.t.n, x, g, first, tile.n, [&](float v, float q) {
+    return up * (__builtin_amdgcn_exp2f((v - m) * c) * inv_s * q_all - q);
+  });
 }
+
+// ---- launches -----------------------------------------------------------------------------------------------------
+// Who works on a row: a wave where its registers hold the row (four rows a workgroup, no barriers), a workgroup of 256
+// threads, or of 1024 - beyond that the row is cut into equal chunks, which a second launch joins.
+constexpr int kWaveVecs = 4, kBlockVecs = 8, kGradVecs = 4;
+constexpr int kWaveList = 64;  // entries of a list that a wave's share of the LDS holds
+struct Plan {
+  int threads;  // 64, 256, 1024
+  Split sp;
+};
+int64_t capacity(int threads, int vecs, int dtype) { return (int64_t)threads * vecs * (dtype == OAKE_F32 ? 4 : 8); }
+Split split(int64_t vocab, int64_t most) {  // equal chunks of at most `most` places, each but the last a multiple of 8
+  const int64_t parts = (vocab + most - 1) / most, chunk = ((vocab + parts - 1) / parts + 7) / 8 * 8;
+  return {chunk, (int)((vocab + chunk - 1) / chunk)};
+}
+Plan forward_plan(int64_t rows, int64_t vocab, int dtype, int list) {
+  if (vocab <= capacity(64, kWaveVecs, dtype) && list <= kWaveList) return {64, {vocab, 1}};
+  if (vocab <= capacity(256, kBlockVecs, dtype)) return {256, {vocab, 1}};
+  return {1024, split(vocab, capacity(1024, kBlockVecs, dtype))};
+}
+Plan backward_plan(int64_t rows, int64_t vocab, int dtype, int list) {
+  if (vocab <= capacity(64, kWaveVecs, dtype) && list <= kWaveList) return {64, {vocab, 1}};
+  return {256, split(vocab, capacity(256, kGradVecs, dtype))};
+}
+dim3 grid_of(int64_t blocks) {
+  const int64_t x = blocks < 1 << 20 ? blocks : 1 << 20;
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+dim3 grid_of(const Plan& p, int64_t rows) { return grid_of(p.threads == 64 ? (rows + 3) / 4 : rows * p.sp.parts); }
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 __attribute__((format(printf, 2, 3))) int refuse(int code, const char* fmt, ...) {
@@ -408,12 +993,65 @@ int launched(const char* what) {
   return e == hipSuccess ? OAKE_OK : refuse(OAKE_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
-#define OAKE_BY_TYPE(dtype, kernel, grid, s, args)                                         \
-  do {                                                                                     \
-    if ((dtype) == OAKE_F32) kernel<float><<<grid, kThreads, 0, s>>>(args);                \
-    else if ((dtype) == OAKE_F16) kernel<f16_t><<<grid, kThreads, 0, s>>>(args);           \
-    else kernel<bf16_t><<<grid, kThreads, 0, s>>>(args);                                   \
+
+template <typename T>
+void run_score(const Plan& p, const ScoreArgs& a, hipStream_t s) {
+  const dim3 grid = grid_of(p, a.r.rows);
+#define OAKE_SCORE(NT, NV)                                                                    \
+  if (a.r.mask) score_kernel<T, NT, NV, true><<<grid, kBlock<NT>, 0, s>>>(a);        \
+  else score_kernel<T, NT, NV, false><<<grid, kBlock<NT>, 0, s>>>(a)
+  if (p.threads == 64) { OAKE_SCORE(64, kWaveVecs); }
+  else if (p.threads == 256) { OAKE_SCORE(256, kBlockVecs); }
+  else { OAKE_SCORE(1024, kBlockVecs); }
+#undef OAKE_SCORE
+  if (a.sp.parts > 1) score_join_kernel<T><<<grid_of(a.r.rows), kThreads, 0, s>>>(a);
+}
+template <typename T>
+void run_score_grad(const Plan& p, const ScoreGradArgs& a, hipStream_t s) {
+  const dim3 grid = grid_of(p, a.r.rows);
+  if (p.threads == 64) {
+    if (a.r.mask) score_grad_kernel<T, 64, kWaveVecs, true, kWaveList><<<grid, 256, 0, s>>>(a);
+    else score_grad_kernel<T, 64, kWaveVecs, false, kWaveList><<<grid, 256, 0, s>>>(a);
+  } else {
+    if (a.r.mask) score_grad_kernel<T, 256, kGradVecs, true, kMaxList + kMaxTop><<<grid, 256, 0, s>>>(a);
+    else score_grad_kernel<T, 256, kGradVecs, false, kMaxList + kMaxTop><<<grid, 256, 0, s>>>(a);
+  }
+}
+template <typename T>
+void run_distill(const Plan& p, const DistillArgs& a, hipStream_t s) {
+  const dim3 grid = grid_of(p, a.r.rows);
+#define OAKE_DISTILL(NT, NV, LIST)                                                                  \
+  if (a.t.tail) distill_kernel<T, NT, NV, true, LIST><<<grid, kBlock<NT>, 0, s>>>(a);      \
+  else distill_kernel<T, NT, NV, false, LIST><<<grid, kBlock<NT>, 0, s>>>(a)
+  if (p.threads == 64) { OAKE_DISTILL(64, kWaveVecs, kWaveList); }
+  else if (p.threads == 256) { OAKE_DISTILL(256, kBlockVecs, kMaxList); }
+  else { OAKE_DISTILL(1024, kBlockVecs, kMaxList); }
+#undef OAKE_DISTILL
+  if (a.sp.parts > 1) distill_join_kernel<T><<<grid_of(a.r.rows), kThreads, 0, s>>>(a);
+}
+template <typename T>
+void run_distill_grad(const Plan& p, const DistillGradArgs& a, hipStream_t s) {
+  const dim3 grid = grid_of(p, a.r.rows);
+  if (p.threads == 64) distill_grad_kernel<T, 64, kWaveVecs, kWaveList><<<grid, 256, 0, s>>>(a);
+  else distill_grad_kernel<T, 256, kGradVecs, kMaxList><<<grid, 256, 0, s>>>(a);
+}
+#define OAKE_BY_TYPE(dtype, run, ...)                       \
+  do {                                                      \
+    if ((dtype) == OAKE_F32) run<float>(__VA_ARGS__);       \
+    else if ((dtype) == OAKE_F16) run<f16_t>(__VA_ARGS__);  \
+    else run<bf16_t>(__VA_ARGS__);                          \
   } while (0)
+
+// scratch of a forward call: [rows, parts, 4] fp32, then [rows, parts, top] keys
+size_t scratch_bytes(int64_t rows, const Split& sp, int top) {
+  return sp.parts == 1 ? 0 : (size_t)rows * sp.parts * (16 + 8 * (size_t)top);
+}
+int check_scratch(const char* what, const void* ws, size_t have, size_t need) {
+  if (need == 0) return OAKE_OK;
+  if (!ws || have < need) return refuse(OAKE_ERR_INVALID, "%s: the workspace has %zu of %zu bytes", what, ws ? have : 0, need);
+  if ((uintptr_t)ws % 16) return refuse(OAKE_ERR_INVALID, "%s: the workspace is not 16-byte aligned", what);
+  return OAKE_OK;
+}
 
 }  // namespace
 }  // namespace oake
@@ -427,7 +1065,7 @@ int oake_logits_workspace(int64_t rows, int64_t vocab, int dtype, int top, size_
   if (!bytes) return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
   if (int rc = check_rows(what, bytes, dtype, rows, vocab, vocab, 1.f)) return rc;
   if (top < 0 || top > kMaxTop) return refuse(OAKE_ERR_INVALID, "%s: top must be 0 .. %d", what, kMaxTop);
-  *bytes = 0;
+  *bytes = scratch_bytes(rows, forward_plan(rows, vocab, dtype, 0).sp, top);
   return OAKE_OK;
 }
 
@@ -443,10 +1081,14 @@ int oake_token_logprobs(const void* d_logits, int dtype, int64_t rows, int64_t v
   if (rows == 0) return OAKE_OK;
   if ((n_targets && (!d_targets || !d_logprobs)) || (top && (!d_top_logprobs || !d_top_indices)))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
-  const ScoreArgs a{{d_logits, rows, vocab, row_stride, d_mask, mask_stride, scale},
+  const Plan p = forward_plan(rows, vocab, dtype, 0);
+  if (int rc = check_scratch(what, d_workspace, workspace_bytes, scratch_bytes(rows, p.sp, top))) return rc;
+  float* sums = static_cast<float*>(d_workspace);
+  uint64_t* keys = p.sp.parts == 1 ? nullptr : reinterpret_cast<uint64_t*>(sums + rows * p.sp.parts * 4);
+  const ScoreArgs a{{d_logits, rows, vocab, row_stride, d_mask, mask_stride, scale}, p.sp,
                     d_targets, index_dtype == OAKE_I64, n_targets, top,
-                    d_logprobs, d_lse, d_entropy, d_top_logprobs, d_stats, d_top_indices};
-  OAKE_BY_TYPE(dtype, score_kernel, (unsigned)rows, (hipStream_t)stream, a);
+                    d_logprobs, d_lse, d_entropy, d_top_logprobs, d_stats, d_top_indices, sums, keys};
+  OAKE_BY_TYPE(dtype, run_score, p, a, (hipStream_t)stream);
   return launched(what);
 }
 
@@ -465,10 +1107,11 @@ int oake_token_logprobs_backward(const void* d_logits, int dtype, int64_t rows, 
   if (int rc = check_grad(what, d_grad, dtype, vocab, rows, grad_stride)) return rc;
   if (!d_stats || (d_grad_logprobs && n_targets && !d_targets) || (d_grad_top && top && !d_top_indices))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
-  const ScoreGradArgs a{{d_logits, rows, vocab, row_stride, d_mask, mask_stride, scale},
+  const Plan p = backward_plan(rows, vocab, dtype, (d_grad_logprobs ? n_targets : 0) + (d_grad_top ? top : 0));
+  const ScoreGradArgs a{{d_logits, rows, vocab, row_stride, d_mask, mask_stride, scale}, p.sp,
                         d_targets, index_dtype == OAKE_I64, n_targets, top, d_top_indices,
                         d_stats, d_grad_logprobs, d_grad_lse, d_grad_entropy, d_grad_top, d_grad, grad_stride};
-  OAKE_BY_TYPE(dtype, score_grad_kernel, (unsigned)rows, (hipStream_t)stream, a);
+  OAKE_BY_TYPE(dtype, run_score_grad, p, a, (hipStream_t)stream);
   return launched(what);
 }
 
@@ -481,9 +1124,12 @@ int oake_distill_top_logits(const void* d_logits, int dtype, int64_t rows, int64
   if (rows == 0) return OAKE_OK;
   if (!d_loss || !d_stats || (top && (!d_top_indices || !d_top_logprobs)))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
-  const DistillArgs a{{d_logits, rows, vocab, row_stride, nullptr, 0, scale},
-                      {d_top_indices, d_top_logprobs, index_dtype == OAKE_I64, top, tail != 0}, d_loss, d_stats};
-  OAKE_BY_TYPE(dtype, distill_kernel, (unsigned)rows, (hipStream_t)stream, a);
+  const Plan p = forward_plan(rows, vocab, dtype, top);
+  if (int rc = check_scratch(what, d_workspace, workspace_bytes, scratch_bytes(rows, p.sp, 0))) return rc;
+  const DistillArgs a{{d_logits, rows, vocab, row_stride, nullptr, 0, scale}, p.sp,
+                      {d_top_indices, d_top_logprobs, index_dtype == OAKE_I64, top, tail != 0}, d_loss, d_stats,
+                      static_cast<float*>(d_workspace)};
+  OAKE_BY_TYPE(dtype, run_distill, p, a, (hipStream_t)stream);
   return launched(what);
 }
 
@@ -498,10 +1144,11 @@ int oake_distill_top_logits_backward(const void* d_logits, int dtype, int64_t ro
   if (int rc = check_grad(what, d_grad, dtype, vocab, rows, grad_stride)) return rc;
   if (!d_stats || !d_grad_loss || (top && (!d_top_indices || !d_top_logprobs)))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
-  const DistillGradArgs a{{d_logits, rows, vocab, row_stride, nullptr, 0, scale},
+  const Plan p = backward_plan(rows, vocab, dtype, top);
+  const DistillGradArgs a{{d_logits, rows, vocab, row_stride, nullptr, 0, scale}, p.sp,
                           {d_top_indices, d_top_logprobs, index_dtype == OAKE_I64, top, tail != 0},
                           d_stats, d_grad_loss, d_grad, grad_stride};
-  OAKE_BY_TYPE(dtype, distill_grad_kernel, (unsigned)rows, (hipStream_t)stream, a);
+  OAKE_BY_TYPE(dtype, run_distill_grad, p, a, (hipStream_t)stream);
   return launched(what);
 }
 
