@@ -59,6 +59,9 @@ typedef u32x4_t u32x4_any __attribute__((aligned(2)));  // at any element's addr
 template <typename T>
 constexpr int kPer = 16 / (int)sizeof(T);
 template <typename T>
+constexpr int kWaveVecs = sizeof(T) == 4 ? 8 : 4;  // of a lane where a wave works on a row
+constexpr int kWavePlaces = 2048;
+template <typename T>
 __device__ __forceinline__ float elem(u32x4_t v, int i) {
   if constexpr (sizeof(T) == 4) return __uint_as_float(v[i]);
   else if constexpr (__is_same(T, f16_t)) return (float)__builtin_bit_cast(f16x8, v)[i];
@@ -78,19 +81,59 @@ __device__ __forceinline__ void drop(u32x4_t& v, int i, bool yes) {  // element 
   }
 }
 
+// x_i * c + d in one operation where the type allows (fp16: the conversion is part of v_fma_mix_f32)
+template <typename T>
+__device__ __forceinline__ float elem_fma(u32x4_t v, int i, float c, float d) {
+  if constexpr (__is_same(T, f16_t)) {
+    float r;
+    if (i & 1) asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(v[i / 2]), "v"(c), "v"(d));
+    else asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(v[i / 2]), "v"(c), "v"(d));
+    return r;
+  } else {
+    return __builtin_fmaf(elem<T>(v, i), c, d);
+  }
+}
+// The largest element.  Three at a time, or two by two in fp16, without the operations that fmaxf spends on signalling
+// NaN: a vector that holds NaN may give any of its elements, or NaN.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float vec_max(u32x4_t v) {
+  if constexpr (sizeof(T) == 4) {
+    const float a = __uint_as_float(v[0]);
+    return max3(max3(a, __uint_as_float(v[1]), __uint_as_float(v[2])), __uint_as_float(v[3]), a);
+  } else if constexpr (__is_same(T, f16_t)) {
+    unsigned a, b;
+    asm("v_pk_max_f16 %0, %1, %2" : "=v"(a) : "v"(v[0]), "v"(v[1]));
+    asm("v_pk_max_f16 %0, %1, %2" : "=v"(b) : "v"(v[2]), "v"(v[3]));
+    asm("v_pk_max_f16 %0, %1, %2" : "=v"(a) : "v"(a), "v"(b));
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 p = __builtin_bit_cast(f16x2, a);
+    return fmaxf((float)p[0], (float)p[1]);
+  } else {
+    float a = max3(elem<T>(v, 0), elem<T>(v, 1), elem<T>(v, 2));
+    a = max3(a, elem<T>(v, 3), elem<T>(v, 4));
+    a = max3(a, elem<T>(v, 5), elem<T>(v, 6));
+    return max3(a, elem<T>(v, 7), a);
+  }
+}
+
 // ---- a group of NT threads: one wave of a 256-thread workgroup (NT 64), or a whole workgroup ---------------------
 template <int NT>
 __device__ __forceinline__ int group_tid() { return NT == 64 ? threadIdx.x % 64 : threadIdx.x; }
 template <int NT>
 constexpr int kBlock = NT == 64 ? 256 : NT;   // threads of a workgroup
 template <int NT>
-constexpr int kWaves = NT == 1024 ? 8 : 4;     // per SIMD, at least: two workgroups a CU
+constexpr int kWaves = 4;                       // per SIMD, at least: two workgroups of 512 a CU
 template <int NT>
 constexpr int kGroups = NT == 64 ? 4 : 1;  // groups of a workgroup
 template <int NT>
 __device__ __forceinline__ int64_t group_index() {
   const int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-  return NT == 64 ? b * 4 + threadIdx.x / 64 : b;
+  return NT == 64 ? b * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : b;  // (scalar: so are the row's addresses)
 }
 template <int NT>
 __device__ __forceinline__ void group_sync() {
@@ -154,7 +197,7 @@ template <typename T, int NT, int NV>
 struct Tile {
   u32x4_t v[NV];
   float single;     // -inf in the threads that have none
-  int nvec, n, nv;
+  int nvec, n, nv;  // whole vectors and places of the chunk; vectors that the thread's wave has any of
 
   // column (within the chunk) of the thread's vector v / single value
   __device__ __forceinline__ int vec_col(int vi) const { return (vi * NT + group_tid<NT>()) * kPer<T>; }
@@ -165,15 +208,12 @@ struct Tile {
   __device__ __forceinline__ void load(const T* x, int count) {
     n = count;
     nvec = n / kPer<T>;
-    nv = (nvec + NT - 1) / NT;
+    const int wave = NT == 64 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x) & ~63;
+    nv = nvec > wave ? (nvec - wave + NT - 1) / NT : 0;
     const u32x4_any* p = reinterpret_cast<const u32x4_any*>(x) + group_tid<NT>();
 #pragma unroll
     for (int vi = 0; vi < NV; ++vi)
-      if (vi < nv) {
-        const unsigned none = neg_inf_bits<T>();
-        v[vi] = u32x4_t{none, none, none, none};
-        if (has_vec(vi)) v[vi] = p[vi * NT];
-      }
+      if (vi < nv && has_vec(vi)) v[vi] = p[vi * NT];
     single = -kInf;
     if (has_single()) single = (float)x[single_col()];
   }
@@ -195,26 +235,46 @@ struct Tile {
 #pragma unroll
     for (int vi = 0; vi < NV; ++vi) asm volatile("" : "+v"(v[vi]));
   }
-  __device__ __forceinline__ float max() const {  // (passes over NaN)
-    float m = single;
+  // f(vector, its first column) for each of the thread's vectors
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
 #pragma unroll
     for (int vi = 0; vi < NV; ++vi)
-      if (vi < nv) {
-#pragma unroll
-        for (int i = 0; i < kPer<T>; ++i) m = fmaxf(m, elem<T>(v[vi], i));
-      }
+      if (vi < nv && has_vec(vi)) f(v[vi], vi);
+  }
+  __device__ __forceinline__ float max() const {
+    float m = single;
+    each([&](u32x4_t q, int) { m = max3(m, vec_max<T>(q), m); });
     return m;
   }
 };
 
-// e_j = 2^((x_j - m) c), m the largest logit, c = scale * log2(e): the difference is taken first, so that e of the largest
-// is exactly 1 (one fused x c - m c would save an operation; measured: no faster).
+// e_j = 2^((x_j - m) c), m the largest logit, c = scale * log2(e).  As it stands this takes two operations beside the
+// exponential; x c - b with b = m c rounded takes one.  That b is off m c by r = m c - b (exact, in a fused multiply-add)
+// multiplies every e_j by 2^r: p = e / S does not see it, and log S is the logarithm of S / 2^r, where 2^r is what the
+// largest logit's own e came out as, so that a row of one place has log p = 0.  (Past |b| = 2^20 r would count: then the
+// plain form.)
+struct Ref {
+  float m, c, b, r, one;
+  bool fused;
+  __device__ __forceinline__ Ref(float max, float c_) : m(max == -kInf ? 0.f : max), c(c_) {  // (-inf: nothing, or only NaN)
+    b = m * c;
+    fused = fabsf(b) < 1048576.f;
+    r = fused ? __builtin_fmaf(m, c, -b) : 0.f;
+    one = __builtin_amdgcn_exp2f(r);
+  }
+};
 struct Sums {
   float s = 0.f, t = 0.f;  // sum e, sum e * log2 e
   __device__ __forceinline__ void add(float d) {
     const float e = __builtin_amdgcn_exp2f(d);
     s += e;
     t += e * fmaxf(d, -200.f);  // 2^-200 is 0 in fp32: a place of probability zero adds 0, not 0 * inf
+  }
+  __device__ __forceinline__ void add_finite(float d) {  // (-inf makes t NaN)
+    const float e = __builtin_amdgcn_exp2f(d);
+    s += e;
+    t = __builtin_fmaf(e, d, t);
   }
 };
 
@@ -233,8 +293,20 @@ __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(
 __device__ __forceinline__ float bound_of(uint32_t prefix) {
   return prefix < 0x00800000u ? -3.402823466e38f : key_value(prefix);  // (-inf is no alternative)
 }
+// (least, largest: of the parts; count(v): how many reach v.)  Halving the interval of keys eight times leaves a 256th of it,
+// which costs about as many keys beyond the top-th; where parts are empty it starts as all numbers and is halved more often.
 template <typename Count>
-__device__ __forceinline__ float bound_by_count(int top, Count count) {
+__device__ __forceinline__ float bound_by_count(float least, float largest, int top, Count count) {
+  uint32_t lo = __builtin_amdgcn_readfirstlane(order_key(least)), hi = __builtin_amdgcn_readfirstlane(order_key(largest)) + 1;
+  for (int left = lo <= kKeyNegInf ? 18 : 8; left > 0; --left) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (count(key_value(mid)) >= top) lo = mid;
+    else hi = mid;
+  }
+  return bound_of(lo);
+}
+template <typename Count>
+__device__ __forceinline__ float bound_by_bits(int top, Count count) {
   uint32_t prefix = 0;
   for (int bit = 31; bit >= 16; --bit)
     if (count(key_value(prefix | 1u << bit)) >= top) prefix |= 1u << bit;
@@ -263,7 +335,7 @@ struct RowStats {
 __device__ __forceinline__ RowStats row_stats(float m, float s, float t) {
   if (s == 0.f) return {m, -kInf, 0.f, 0.f};
   const float log_s = logf(s);
-  return {m, log_s, log_s - t / s * kLn2, 1.f / s};
+  return {m, log_s, log_s - fminf(t / s, 0.f) * kLn2, 1.f / s};
 }
 __device__ __forceinline__ void write_row(const ScoreArgs& a, int64_t row, const RowStats& st) {
   if (a.lse) a.lse[row] = st.log_s == -kInf ? -kInf : st.m * a.r.scale + st.log_s;
@@ -275,16 +347,28 @@ __device__ __forceinline__ void write_row(const ScoreArgs& a, int64_t row, const
     a.stats[row * 4 + 3] = st.inv_s;
   }
 }
+// Given tokens: the first of each thread is fetched while the row is (its logit is two loads away), the others at the end.
 template <typename T>
-__device__ __forceinline__ void write_given(const ScoreArgs& a, int64_t row, const RowStats& st, int t, int threads) {
-  const T* x = static_cast<const T*>(a.r.x) + row * a.r.stride;
-  const uint8_t* mask = a.r.mask ? a.r.mask + row * a.r.mask_stride : nullptr;
+__device__ __forceinline__ float given_logit(const ScoreArgs& a, int64_t row, int64_t j) {  // NaN: no such token
+  if (j < 0 || j >= a.r.vocab) return __builtin_nanf("");
+  if (a.r.mask && !a.r.mask[row * a.r.mask_stride + j]) return -kInf;
+  return (float)static_cast<const T*>(a.r.x)[row * a.r.stride + j];
+}
+struct Given {
+  int64_t id;
+  float x;
+};
+__device__ __forceinline__ int64_t given_id(const ScoreArgs& a, int64_t row, int i) {
+  return i < a.n_targets ? load_id(a.targets, a.wide_ids, row * a.n_targets + i) : -1;
+}
+template <typename T>
+__device__ __forceinline__ void write_given(const ScoreArgs& a, int64_t row, const RowStats& st, int t, int threads, Given g) {
   for (int i = t; i < a.n_targets; i += threads) {
-    const int64_t j = load_id(a.targets, a.wide_ids, row * a.n_targets + i);
-    float v = 0.f;
-    if (j >= a.r.vocab) v = __builtin_nanf("");
-    else if (j >= 0) v = logp_at(mask && !mask[j] ? -kInf : (float)x[j], st.m, st.log_s, a.r.scale);
-    a.logprobs[row * a.n_targets + i] = v;
+    if (i != t) {
+      g.id = given_id(a, row, i);
+      g.x = given_logit<T>(a, row, g.id);
+    }
+    a.logprobs[row * a.n_targets + i] = g.id < 0 ? 0.f : logp_at(g.x, st.m, st.log_s, a.r.scale);
   }
 }
 __device__ __forceinline__ void write_top(const ScoreArgs& a, int64_t row, const RowStats& st, int rank, uint64_t key) {
@@ -304,33 +388,42 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
   __shared__ int list_n[G];
   const int64_t index = group_index<NT>();
   if (index >= a.r.rows * a.sp.parts) return;
-  const int64_t row = index / a.sp.parts;
+  const int64_t row = a.sp.parts == 1 ? index : index / a.sp.parts;
   const int part = (int)(index - row * a.sp.parts);
   const int g = NT == 64 ? threadIdx.x / 64 : 0, t = group_tid<NT>();
   const int64_t first = part * a.sp.chunk;
   const int64_t left = a.r.vocab - first;
   const T* x = static_cast<const T*>(a.r.x) + row * a.r.stride + first;
+  const bool whole = a.sp.parts == 1;
+  Given given;
+  given.id = whole ? given_id(a, row, t) : -1;
   Tile<T, NT, NV> tile;
   tile.load(x, (int)(left < a.sp.chunk ? left : a.sp.chunk));
+  given.x = given.id < 0 ? 0.f : given_logit<T>(a, row, given.id);
   if constexpr (MASK) tile.apply_mask(a.r.mask + row * a.r.mask_stride + first);
   if (t == 0) list_n[g] = 0;
 
   // the largest logit, and a bound for the alternatives
-  float mine = tile.max(), m, bound = kInf;
+  float vmax[NV], mine = tile.single, m, bound = kInf;
+  tile.each([&](u32x4_t q, int vi) {
+    vmax[vi] = vec_max<T>(q);
+    mine = max3(mine, vmax[vi], vmax[vi]);
+  });
   if constexpr (NT == 64) {
     m = wave64_max(mine);
     if (a.top) {
       // parts: the lanes' own places where enough of them have any; else each place for itself
       if (a.top <= 32 && tile.nvec >= 2 * a.top) {
-        bound = bound_by_count(a.top, [&](float v) { return __popcll(__ballot(mine >= v)); });
+        bound = bound_by_bits(a.top, [&](float v) { return __popcll(__ballot(mine >= v)); });
       } else {
-        bound = bound_by_count(a.top, [&](float v) {
+        bound = bound_by_bits(a.top, [&](float v) {
           int n = __popcll(__ballot(tile.single >= v));
 #pragma unroll
           for (int vi = 0; vi < NV; ++vi)
             if (vi < tile.nv) {
+              const bool here = tile.has_vec(vi);
 #pragma unroll
-              for (int i = 0; i < E; ++i) n += __popcll(__ballot(elem<T>(tile.v[vi], i) >= v));
+              for (int i = 0; i < E; ++i) n += __popcll(__ballot(here && elem<T>(tile.v[vi], i) >= v));
             }
           return n;
         });
@@ -345,68 +438,85 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
     __syncthreads();
     const float4 q = *reinterpret_cast<const float4*>(&part_max[t % 64 * 4]);
     m = wave64_max(fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)));
-    if (a.top)
-      bound = bound_by_count(a.top, [&](float v) {
-        return __popcll(__ballot(q.x >= v)) + __popcll(__ballot(q.y >= v)) + __popcll(__ballot(q.z >= v)) +
-               __popcll(__ballot(q.w >= v));
-      });
+    if (a.top) {
+      const float four = fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w));
+      if (a.top <= 32) {
+        bound = bound_by_count(-wave64_max(-four), m, a.top, [&](float v) { return __popcll(__ballot(four >= v)); });
+      } else {
+        const float least = -wave64_max(-fminf(fminf(q.x, q.y), fminf(q.z, q.w)));
+        bound = bound_by_count(least, m, a.top, [&](float v) {
+          return __popcll(__ballot(q.x >= v)) + __popcll(__ballot(q.y >= v)) + __popcll(__ballot(q.z >= v)) +
+                 __popcll(__ballot(q.w >= v));
+        });
+      }
+    }
   }
 
   // sums, and the places at or above the bound
+  const Ref ref(m, a.r.scale * kLog2e);
+  m = ref.m;
   tile.pack();
-  if (m == -kInf) m = 0.f;  // nothing allowed (the sum is 0), or nothing but NaN (the sum is NaN)
-  const float c = a.r.scale * kLog2e;
   Sums sums;
   const auto keep = [&](float v, int col) {
     const int at = atomicAdd(&list_n[g], 1);
     if (at < CAP) list[g][at] = place_key(v, (uint32_t)(first + col));
   };
   if constexpr (NT == 64) group_sync<NT>();  // (list_n is 0)
+  tile.each([&](u32x4_t q, int vi) {
 #pragma unroll
-  for (int vi = 0; vi < NV; ++vi)
-    if (vi < tile.nv) {
-      float best = -kInf;
+    for (int i = 0; i < E; ++i) {
+      const float d = elem_fma<T>(q, i, ref.c, -ref.b);
+      if constexpr (MASK) sums.add(d);
+      else sums.add_finite(d);
+    }
+    if (vmax[vi] >= bound) {
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const float v = elem<T>(tile.v[vi], i);
-        best = fmaxf(best, v);
-        sums.add((v - m) * c);
-      }
-      if (best >= bound) {
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const float v = elem<T>(tile.v[vi], i);
-          if (v >= bound) keep(v, tile.vec_col(vi) + i);
-        }
+        const float v = elem<T>(q, i);
+        if (v >= bound) keep(v, tile.vec_col(vi) + i);
       }
     }
-  sums.add((tile.single - m) * c);
+  });
+  sums.add(__builtin_fmaf(tile.single, ref.c, -ref.b));
   if (tile.single >= bound) keep(tile.single, tile.single_col());
-  sums.s = wave64_sum(sums.s);
-  sums.t = wave64_sum(sums.t);
-  if constexpr (NT == 64) {
-    group_sync<NT>();
-  } else {
-    if (t % 64 == 0) {
-      tmp_s[t / 64] = sums.s;
-      tmp_t[t / 64] = sums.t;
-    }
-    __syncthreads();
-    sums.s = tmp_s[0];
-    sums.t = tmp_t[0];
+  const auto reduce = [&]() {
+    sums.s = wave64_sum(sums.s);
+    sums.t = wave64_sum(sums.t);
+    if constexpr (NT == 64) {
+      group_sync<NT>();
+    } else {
+      if (t % 64 == 0) {
+        tmp_s[t / 64] = sums.s;
+        tmp_t[t / 64] = sums.t;
+      }
+      __syncthreads();
+      sums.s = tmp_s[0];
+      sums.t = tmp_t[0];
 #pragma unroll
-    for (int w = 1; w < NT / 64; ++w) {
-      sums.s += tmp_s[w];
-      sums.t += tmp_t[w];
+      for (int w = 1; w < NT / 64; ++w) {
+        sums.s += tmp_s[w];
+        sums.t += tmp_t[w];
+      }
     }
+  };
+  reduce();
+  const uint8_t* mask = MASK ? a.r.mask + row * a.r.mask_stride + first : nullptr;
+  if (!ref.fused || (sums.t != sums.t && sums.s == sums.s)) {
+    // logits past what the fused form takes, or -inf among them: again, from memory
+    if constexpr (NT != 64) __syncthreads();
+    sums = Sums();
+    for (int j = t; j < tile.n; j += NT) sums.add(((MASK && !mask[j] ? -kInf : (float)x[j]) - m) * ref.c);
+    reduce();
+  } else {  // relative to m
+    sums.s /= ref.one;
+    sums.t = sums.t / ref.one - ref.r * sums.s;
   }
 
   RowStats st;
-  const bool whole = a.sp.parts == 1;
   if (whole) {
     st = row_stats(m, sums.s, sums.t);
     if (t == 0) write_row(a, row, st);
-    write_given<T>(a, row, st, t, NT);
+    write_given<T>(a, row, st, t, NT, given);
   } else if (t == 0) {
     float* p = a.part_sums + index * 4;
     p[0] = m;
@@ -426,8 +536,11 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
       int rank = 0;
 #pragma unroll 8
       for (int k = t % R; k < n; k += R) rank += list[g][k] > key;
-#pragma unroll
-      for (int o = 1; o < R; o *= 2) rank += __shfl_xor(rank, o, 64);
+      rank += __builtin_amdgcn_update_dpp(0, rank, 0xB1, 0xF, 0xF, true);              // quad_perm 1 0 3 2
+      if constexpr (R == 8) {
+        rank += __builtin_amdgcn_update_dpp(0, rank, 0x4E, 0xF, 0xF, true);            // quad_perm 2 3 0 1
+        rank += __builtin_amdgcn_update_dpp(0, rank, 0x141, 0xF, 0xF, true);           // row_half_mirror
+      }
       if (t % R == 0 && rank < a.top) put(rank, key);
     }
     for (int i = n + t; i < a.top; i += NT) put(i, 0);
@@ -435,7 +548,6 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
   }
   // (from memory again: the tile's registers are not held for the rare case)
   uint64_t last = ~0ull;
-  const uint8_t* mask = MASK ? a.r.mask + row * a.r.mask_stride + first : nullptr;
   for (int i = 0; i < a.top; ++i) {
     uint64_t best = 0;
     for (int j = t; j < tile.n; j += NT) {
@@ -465,6 +577,9 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
   const int t = threadIdx.x, parts = a.sp.parts, top = a.top;
   const float* p = a.part_sums + row * parts * 4;
   const float c = a.r.scale * kLog2e;
+  Given given;
+  given.id = given_id(a, row, t);
+  given.x = given.id < 0 ? 0.f : given_logit<T>(a, row, given.id);
   // every wave for itself: no exchange
   float m = -kInf, s = 0.f, u = 0.f;
   for (int i = t % 64; i < parts; i += 64)
@@ -482,7 +597,7 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
   u = wave64_sum(u);
   const RowStats st = row_stats(m, s, u);
   if (t == 0) write_row(a, row, st);
-  write_given<T>(a, row, st, t, kThreads);
+  write_given<T>(a, row, st, t, kThreads, given);
   if (top == 0) return;
 
   const int64_t total = (int64_t)parts * top;
@@ -669,7 +784,7 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
   __shared__ float tmp_m[NT / 64], tmp_s[NT / 64], tmp_l[NT / 64];
   const int64_t index = group_index<NT>();
   if (index >= a.r.rows * a.sp.parts) return;
-  const int64_t row = index / a.sp.parts;
+  const int64_t row = a.sp.parts == 1 ? index : index / a.sp.parts;
   const int part = (int)(index - row * a.sp.parts);
   const int g = NT == 64 ? threadIdx.x / 64 : 0, t = group_tid<NT>();
   const int64_t first = part * a.sp.chunk;
@@ -698,7 +813,7 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
     group_sync<NT>();
 #pragma unroll
     for (int vi = 0; vi < NV; ++vi)
-      if (vi < tile.nv) {
+      if (vi < tile.nv && tile.has_vec(vi)) {
         const int q = vi * NT + t;
         const unsigned bits = map[g][q * E / 32] >> q * E % 32 & ((1u << E) - 1);
         if (bits) {
@@ -721,17 +836,24 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
     if (t == 0 && whole) write_no_teacher(a, row);
     return;
   }
-  if (m == -kInf) m = 0.f;
-  const float c = a.r.scale * kLog2e;
-  float s = __builtin_amdgcn_exp2f((tile.single - m) * c);
+  const Ref ref(m, a.r.scale * kLog2e);
+  m = ref.m;
   tile.pack();
+  float s = 0.f;
+  if (ref.fused) {
+    tile.each([&](u32x4_t q, int) {
 #pragma unroll
-  for (int vi = 0; vi < NV; ++vi)
-    if (vi < tile.nv) {
+      for (int i = 0; i < E; ++i) s += __builtin_amdgcn_exp2f(elem_fma<T>(q, i, ref.c, -ref.b));
+    });
+    s += __builtin_amdgcn_exp2f(__builtin_fmaf(tile.single, ref.c, -ref.b));
+  } else {
+    tile.each([&](u32x4_t q, int) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) s += __builtin_amdgcn_exp2f((elem<T>(tile.v[vi], i) - m) * c);
-    }
-  s = group_sum<NT>(s, tmp_s);
+      for (int i = 0; i < E; ++i) s += __builtin_amdgcn_exp2f((elem<T>(q, i) - m) * ref.c);
+    });
+    s += __builtin_amdgcn_exp2f((tile.single - m) * ref.c);
+  }
+  s = group_sum<NT>(s, tmp_s) / ref.one;
   if (whole) {
     finish_distill<T, NT>(a, row, te[g], TAIL && !twice[g], m, s, tmp_l);
   } else if (t == 0) {
@@ -826,7 +948,7 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_grad_kernel(Scor
   __shared__ float tmp[NT / 64];
   const int64_t index = group_index<NT>();
   if (index >= a.r.rows * a.sp.parts) return;
-  const int64_t row = index / a.sp.parts;
+  const int64_t row = a.sp.parts == 1 ? index : index / a.sp.parts;
   const int64_t first = (index - row * a.sp.parts) * a.sp.chunk;
   const int64_t left = a.r.vocab - first;
   const T* xr = static_cast<const T*>(a.r.x) + row * a.r.stride;
@@ -891,7 +1013,7 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_grad_kernel(Di
   __shared__ float ws[G][LIST];
   const int64_t index = group_index<NT>();
   if (index >= a.r.rows * a.sp.parts) return;
-  const int64_t row = index / a.sp.parts;
+  const int64_t row = a.sp.parts == 1 ? index : index / a.sp.parts;
   const int64_t first = (index - row * a.sp.parts) * a.sp.chunk;
   const int64_t left = a.r.vocab - first;
   const T* x = static_cast<const T*>(a.r.x) + row * a.r.stride + first;
@@ -926,10 +1048,10 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_grad_kernel(Di
 // ---- launches -----------------------------------------------------------------------------------------------------
 // Who works on a row: a wave where its registers hold the row (four rows a workgroup, no barriers), a workgroup of 256
 // threads, or of 1024 - beyond that the row is cut into equal chunks, which a second launch joins.
-constexpr int kWaveVecs = 4, kBlockVecs = 8, kGradVecs = 4;
+constexpr int kBlockVecs = 8, kLongVecs = 16, kGradVecs = 4;
 constexpr int kWaveList = 64;  // entries of a list that a wave's share of the LDS holds
 struct Plan {
-  int threads;  // 64, 256, 1024
+  int threads;  // 64, 256, 512
   Split sp;
 };
 int64_t capacity(int threads, int vecs, int dtype) { return (int64_t)threads * vecs * (dtype == OAKE_F32 ? 4 : 8); }
@@ -938,12 +1060,12 @@ Split split(int64_t vocab, int64_t most) {  // equal chunks of at most `most` pl
   return {chunk, (int)((vocab + chunk - 1) / chunk)};
 }
 Plan forward_plan(int64_t rows, int64_t vocab, int dtype, int list) {
-  if (vocab <= capacity(64, kWaveVecs, dtype) && list <= kWaveList) return {64, {vocab, 1}};
+  if (vocab <= kWavePlaces && list <= kWaveList) return {64, {vocab, 1}};
   if (vocab <= capacity(256, kBlockVecs, dtype)) return {256, {vocab, 1}};
-  return {1024, split(vocab, capacity(1024, kBlockVecs, dtype))};
+  return {512, split(vocab, capacity(512, kLongVecs, dtype))};
 }
 Plan backward_plan(int64_t rows, int64_t vocab, int dtype, int list) {
-  if (vocab <= capacity(64, kWaveVecs, dtype) && list <= kWaveList) return {64, {vocab, 1}};
+  if (vocab <= kWavePlaces && list <= kWaveList) return {64, {vocab, 1}};
   return {256, split(vocab, capacity(256, kGradVecs, dtype))};
 }
 dim3 grid_of(int64_t blocks) {
@@ -1000,9 +1122,9 @@ void run_score(const Plan& p, const ScoreArgs& a, hipStream_t s) {
 #define OAKE_SCORE(NT, NV)                                                                    \
   if (a.r.mask) score_kernel<T, NT, NV, true><<<grid, kBlock<NT>, 0, s>>>(a);        \
   else score_kernel<T, NT, NV, false><<<grid, kBlock<NT>, 0, s>>>(a)
-  if (p.threads == 64) { OAKE_SCORE(64, kWaveVecs); }
+  if (p.threads == 64) { OAKE_SCORE(64, kWaveVecs<T>); }
   else if (p.threads == 256) { OAKE_SCORE(256, kBlockVecs); }
-  else { OAKE_SCORE(1024, kBlockVecs); }
+  else { OAKE_SCORE(512, kLongVecs); }
 #undef OAKE_SCORE
   if (a.sp.parts > 1) score_join_kernel<T><<<grid_of(a.r.rows), kThreads, 0, s>>>(a);
 }
@@ -1010,8 +1132,8 @@ template <typename T>
 void run_score_grad(const Plan& p, const ScoreGradArgs& a, hipStream_t s) {
   const dim3 grid = grid_of(p, a.r.rows);
   if (p.threads == 64) {
-    if (a.r.mask) score_grad_kernel<T, 64, kWaveVecs, true, kWaveList><<<grid, 256, 0, s>>>(a);
-    else score_grad_kernel<T, 64, kWaveVecs, false, kWaveList><<<grid, 256, 0, s>>>(a);
+    if (a.r.mask) score_grad_kernel<T, 64, kWaveVecs<T>, true, kWaveList><<<grid, 256, 0, s>>>(a);
+    else score_grad_kernel<T, 64, kWaveVecs<T>, false, kWaveList><<<grid, 256, 0, s>>>(a);
   } else {
     if (a.r.mask) score_grad_kernel<T, 256, kGradVecs, true, kMaxList + kMaxTop><<<grid, 256, 0, s>>>(a);
     else score_grad_kernel<T, 256, kGradVecs, false, kMaxList + kMaxTop><<<grid, 256, 0, s>>>(a);
@@ -1023,16 +1145,16 @@ void run_distill(const Plan& p, const DistillArgs& a, hipStream_t s) {
 #define OAKE_DISTILL(NT, NV, LIST)                                                                  \
   if (a.t.tail) distill_kernel<T, NT, NV, true, LIST><<<grid, kBlock<NT>, 0, s>>>(a);      \
   else distill_kernel<T, NT, NV, false, LIST><<<grid, kBlock<NT>, 0, s>>>(a)
-  if (p.threads == 64) { OAKE_DISTILL(64, kWaveVecs, kWaveList); }
+  if (p.threads == 64) { OAKE_DISTILL(64, kWaveVecs<T>, kWaveList); }
   else if (p.threads == 256) { OAKE_DISTILL(256, kBlockVecs, kMaxList); }
-  else { OAKE_DISTILL(1024, kBlockVecs, kMaxList); }
+  else { OAKE_DISTILL(512, kLongVecs, kMaxList); }
 #undef OAKE_DISTILL
   if (a.sp.parts > 1) distill_join_kernel<T><<<grid_of(a.r.rows), kThreads, 0, s>>>(a);
 }
 template <typename T>
 void run_distill_grad(const Plan& p, const DistillGradArgs& a, hipStream_t s) {
   const dim3 grid = grid_of(p, a.r.rows);
-  if (p.threads == 64) distill_grad_kernel<T, 64, kWaveVecs, kWaveList><<<grid, 256, 0, s>>>(a);
+  if (p.threads == 64) distill_grad_kernel<T, 64, kWaveVecs<T>, kWaveList><<<grid, 256, 0, s>>>(a);
   else distill_grad_kernel<T, 256, kGradVecs, kMaxList><<<grid, 256, 0, s>>>(a);
 }
 #define OAKE_BY_TYPE(dtype, run, ...)                       \
