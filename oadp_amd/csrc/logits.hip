@@ -289,21 +289,44 @@ __device__ __forceinline__ float logp_at(float x, float m, float log_s, float sc
 // wave's lanes; the places at or above it go to a list in LDS as keys, and each key's rank is the number of larger ones.
 // 49408 normal logits, 256 parts, top 20: about 21 keys.  A list that overflows (crowded equal values) or a row with
 // NaN (which the maxima pass over) is worked off one alternative at a time instead.
+constexpr float kLowest = -3.402823466e38f;
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ float bound_of(uint32_t prefix) {
-  return prefix < 0x00800000u ? -3.402823466e38f : key_value(prefix);  // (-inf is no alternative)
+  return prefix < 0x00800000u ? kLowest : key_value(prefix);  // (-inf is no alternative)
 }
-// (least, largest: of the parts; count(v): how many reach v.)  Halving the interval of keys eight times leaves a 256th of it,
-// which costs about as many keys beyond the top-th; where parts are empty it starts as all numbers and is halved more often.
+// (least, largest: of the parts; count(v): how many reach v.)  Eight halvings of the interval of values, then, where that has
+// left too many parts - values of very different sizes, parts that are empty - halvings by key and by value in turn.
 template <typename Count>
 __device__ __forceinline__ float bound_by_count(float least, float largest, int top, Count count) {
-  uint32_t lo = __builtin_amdgcn_readfirstlane(order_key(least)), hi = __builtin_amdgcn_readfirstlane(order_key(largest)) + 1;
-  for (int left = lo <= kKeyNegInf ? 18 : 8; left > 0; --left) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    if (count(key_value(mid)) >= top) lo = mid;
-    else hi = mid;
+  float lo = least, hi = largest;
+  int reached = 1 << 20;
+  if (least > -kInf) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float mid = 0.5f * lo + 0.5f * hi;
+      const int n = count(mid);
+      const bool up = n >= top;
+      reached = up ? n : reached;
+      lo = up ? mid : lo;
+      hi = up ? hi : mid;
+    }
   }
-  return bound_of(lo);
+  if (reached > 2 * top + 16) {
+    uint32_t a = __builtin_amdgcn_readfirstlane(order_key(lo)), b = __builtin_amdgcn_readfirstlane(order_key(hi)) + 1;
+    for (int i = 0; i < 32 && b - a > 1; ++i) {
+      uint32_t mid = a + (b - a) / 2;
+      if (i % 2 && a > kKeyNegInf) {
+        const uint32_t k = __builtin_amdgcn_readfirstlane(order_key(0.5f * key_value(a) + 0.5f * key_value(b)));
+        mid = k > a && k < b ? k : mid;
+      }
+      const int n = count(key_value(mid));
+      if (n >= top) a = mid;
+      else b = mid;
+      if (n >= top && n <= top + top / 8 + 2) break;
+    }
+    lo = a <= kKeyNegInf ? kLowest : key_value(a);
+  }
+  return lo;
 }
 template <typename Count>
 __device__ __forceinline__ float bound_by_bits(int top, Count count) {
@@ -314,7 +337,9 @@ __device__ __forceinline__ float bound_by_bits(int top, Count count) {
 }
 constexpr int kParts = 256;  // maxima of a workgroup's parts
 template <int NT>
-constexpr int kListCap = NT == 64 ? 256 : 1024;
+constexpr int kListCap = NT == 64 ? 256 : 1024;  // keys
+template <int NT>
+constexpr int kVecCap = NT == 64 ? 96 : 512;     // vectors that hold some
 
 // ---- token_logprobs -----------------------------------------------------------------------------------------
 struct ScoreArgs {
@@ -384,6 +409,9 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
   __shared__ __attribute__((aligned(16))) float part_max[NT == 64 ? 1 : kParts];
   __shared__ float tmp_s[NT / 64], tmp_t[NT / 64];
   __shared__ uint64_t tmp_k[NT / 64];
+  constexpr int VECS = kVecCap<NT>;
+  __shared__ u32x4_t vecs[G][VECS];
+  __shared__ int vec_col[G][VECS], vecs_n[G];
   __shared__ uint64_t list[G][CAP];
   __shared__ int list_n[G];
   const int64_t index = group_index<NT>();
@@ -401,7 +429,7 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
   tile.load(x, (int)(left < a.sp.chunk ? left : a.sp.chunk));
   given.x = given.id < 0 ? 0.f : given_logit<T>(a, row, given.id);
   if constexpr (MASK) tile.apply_mask(a.r.mask + row * a.r.mask_stride + first);
-  if (t == 0) list_n[g] = 0;
+  if (t == 0) vecs_n[g] = list_n[g] = 0;
 
   // the largest logit, and a bound for the alternatives
   float vmax[NV], mine = tile.single, m, bound = kInf;
@@ -457,9 +485,12 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
   m = ref.m;
   tile.pack();
   Sums sums;
-  const auto keep = [&](float v, int col) {
-    const int at = atomicAdd(&list_n[g], 1);
-    if (at < CAP) list[g][at] = place_key(v, (uint32_t)(first + col));
+  const auto keep = [&](u32x4_t q, int col) {  // a vector that holds places at or above the bound
+    const int at = atomicAdd(&vecs_n[g], 1);
+    if (at < VECS) {
+      vecs[g][at] = q;
+      vec_col[g][at] = col;
+    }
   };
   if constexpr (NT == 64) group_sync<NT>();  // (list_n is 0)
   tile.each([&](u32x4_t q, int vi) {
@@ -469,16 +500,16 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
       if constexpr (MASK) sums.add(d);
       else sums.add_finite(d);
     }
-    if (vmax[vi] >= bound) {
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const float v = elem<T>(q, i);
-        if (v >= bound) keep(v, tile.vec_col(vi) + i);
-      }
-    }
+    if (vmax[vi] >= bound) keep(q, tile.vec_col(vi));
   });
   sums.add(__builtin_fmaf(tile.single, ref.c, -ref.b));
-  if (tile.single >= bound) keep(tile.single, tile.single_col());
+  if (tile.single >= bound) {
+    const unsigned none = neg_inf_bits<T>();
+    u32x4_t q = u32x4_t{none, none, none, none};
+    if constexpr (sizeof(T) == 4) q[0] = __float_as_uint(tile.single);
+    else q[0] = (none & 0xFFFF0000u) | __builtin_bit_cast(unsigned short, to16<T>(tile.single));
+    keep(q, tile.single_col());
+  }
   const auto reduce = [&]() {
     sums.s = wave64_sum(sums.s);
     sums.t = wave64_sum(sums.t);
@@ -528,8 +559,20 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
     if (whole) write_top(a, row, st, rank, key);
     else a.part_keys[index * a.top + rank] = key;
   };
+  const int held = vecs_n[g];
+  if (held <= VECS) {  // the places of those vectors, all threads at once
+    const T* all = reinterpret_cast<const T*>(vecs[g]);
+    for (int i = t; i < held * E; i += NT) {
+      const float v = (float)all[i];
+      if (v >= bound) {
+        const int at = atomicAdd(&list_n[g], 1);
+        if (at < CAP) list[g][at] = place_key(v, (uint32_t)(first + vec_col[g][i / E] + i % E));
+      }
+    }
+  }
+  group_sync<NT>();
   const int n = list_n[g];
-  if (n <= CAP && sums.s == sums.s) {
+  if (held <= VECS && n <= CAP && sums.s == sums.s) {
     constexpr int R = NT == 64 ? 2 : 8;  // lanes that count for one key
     for (int i = t / R; i < n; i += NT / R) {
       const uint64_t key = list[g][i];
@@ -603,21 +646,30 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
   const int64_t total = (int64_t)parts * top;
   const uint64_t* all = a.part_keys + row * total;
   int some = 0;  // alternatives of the row that this thread has seen: the rest of the answer is filled up
+  const int share = (top + parts - 1) / parts - 1;
   const auto merge = [&](const uint64_t* keys) {
+    // of every list its share'th key: at least `top` keys reach the least of these
+    uint64_t bound = ~0ull;
+    for (int p = 0; p < parts; ++p) {
+      const uint64_t k = keys[(int64_t)p * top + share];
+      bound = k < bound ? k : bound;
+    }
     for (int64_t i = t; i < total; i += kThreads) {
       const uint64_t key = keys[i];
-      if (key == 0) continue;
-      ++some;
+      some += key != 0;
+      if (key == 0 || key < bound) continue;
       const int own = (int)(i / top);
       int64_t rank = i - (int64_t)own * top;
-#pragma unroll 4
+#pragma unroll 8
       for (int p = 0; p < parts; ++p) {
-        if (p == own) continue;
         const uint64_t* other = keys + (int64_t)p * top;
         int lo = 0;  // keys of the other list before `lo` are larger
-        for (int step = kMaxTop; step > 0; step /= 2)
-          if (lo + step <= top && other[lo + step - 1] > key) lo += step;
-        rank += lo;
+#pragma unroll
+        for (int step = kMaxTop; step > 0; step /= 2) {
+          const int at = lo + step < top ? lo + step : top;
+          lo = other[at - 1] > key ? at : lo;
+        }
+        rank += p == own ? 0 : lo;
       }
       if (rank < top) write_top(a, row, st, (int)rank, key);
     }
