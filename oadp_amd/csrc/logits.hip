@@ -44,6 +44,7 @@ struct Rows {  // rows of logits and what of them is allowed
   const uint8_t* mask;   // nullptr: everything; else 1 byte a logit, 0 = not allowed
   int64_t mask_stride;   // 0: one mask for all rows
   float scale;
+  bool big;              // more than the Infinity Cache holds: read past it
 };
 struct Split {           // a row as `parts` chunks of `chunk` places, each a workgroup's (or a wave's) own
   int64_t chunk;
@@ -205,15 +206,24 @@ struct Tile {
   __device__ __forceinline__ bool has_single() const { return group_tid<NT>() < n - nvec * kPer<T>; }
   __device__ __forceinline__ bool has_vec(int vi) const { return vi * NT + group_tid<NT>() < nvec; }
 
-  __device__ __forceinline__ void load(const T* x, int count) {
+  __device__ __forceinline__ void load(const T* x, int count, bool past_cache) {
     n = count;
     nvec = n / kPer<T>;
     const int wave = NT == 64 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x) & ~63;
     nv = nvec > wave ? (nvec - wave + NT - 1) / NT : 0;
     const u32x4_any* p = reinterpret_cast<const u32x4_any*>(x) + group_tid<NT>();
+    if (past_cache) {
 #pragma unroll
-    for (int vi = 0; vi < NV; ++vi)
-      if (vi < nv && has_vec(vi)) v[vi] = p[vi * NT];
+      for (int vi = 0; vi < NV; ++vi)
+        if (vi < nv && has_vec(vi)) {
+          v[vi] = __builtin_nontemporal_load(p + vi * NT);
+          asm volatile("");  // (or the compiler makes one plain access of the two)
+        }
+    } else {
+#pragma unroll
+      for (int vi = 0; vi < NV; ++vi)
+        if (vi < nv && has_vec(vi)) v[vi] = p[vi * NT];
+    }
     single = -kInf;
     if (has_single()) single = (float)x[single_col()];
   }
@@ -426,7 +436,7 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
   Given given;
   given.id = whole ? given_id(a, row, t) : -1;
   Tile<T, NT, NV> tile;
-  tile.load(x, (int)(left < a.sp.chunk ? left : a.sp.chunk));
+  tile.load(x, (int)(left < a.sp.chunk ? left : a.sp.chunk), a.r.big);
   given.x = given.id < 0 ? 0.f : given_logit<T>(a, row, given.id);
   if constexpr (MASK) tile.apply_mask(a.r.mask + row * a.r.mask_stride + first);
   if (t == 0) vecs_n[g] = list_n[g] = 0;
@@ -844,7 +854,7 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
   const T* x = static_cast<const T*>(a.r.x) + row * a.r.stride + first;
   const bool whole = a.sp.parts == 1;
   Tile<T, NT, NV> tile;
-  tile.load(x, (int)(left < a.sp.chunk ? left : a.sp.chunk));
+  tile.load(x, (int)(left < a.sp.chunk ? left : a.sp.chunk), a.r.big);
   if (t == 0) twice[g] = 0;
   if constexpr (TAIL) {
     for (int i = t; i < WORDS; i += NT) map[g][i] = 0;
@@ -945,7 +955,7 @@ __global__ __launch_bounds__(kThreads) void distill_join_kernel(DistillArgs a) {
 // entries that name j.  A chunk is written whole first, then its listed places again, each by the first entry that names
 // it with the weights of all of them, so that no sum depends on an order.
 template <typename T, int NT, int NV, typename F>
-__device__ __forceinline__ void write_dense(const Tile<T, NT, NV>& tile, T* g, F value) {
+__device__ __forceinline__ void write_dense(const Tile<T, NT, NV>& tile, T* g, bool past_cache, F value) {
 #pragma unroll
   for (int vi = 0; vi < NV; ++vi)
     if (vi < tile.nv && tile.has_vec(vi)) {
@@ -959,7 +969,9 @@ __device__ __forceinline__ void write_dense(const Tile<T, NT, NV>& tile, T* g, F
         for (int i = 0; i < 8; ++i) o[i] = to16<T>(value(elem<T>(tile.v[vi], i)));
         out = __builtin_bit_cast(u32x4_t, o);
       }
-      *reinterpret_cast<u32x4_any*>(g + tile.vec_col(vi)) = out;
+      u32x4_any* to = reinterpret_cast<u32x4_any*>(g + tile.vec_col(vi));
+      if (past_cache) store16_policy<2>(g + tile.vec_col(vi), out);  // (nt; any alignment)
+      else *to = out;
     }
   if (tile.has_single()) g[tile.single_col()] = to16<T>(value(tile.single));
 }
@@ -990,6 +1002,7 @@ struct ScoreGradArgs {
   const float *stats, *g_logprobs, *g_lse, *g_entropy, *g_top;
   void* grad;
   int64_t grad_stride;
+  bool write_past;       // the gradient goes past the cache
 };
 
 template <typename T, int NT, int NV, bool MASK, int LIST>
@@ -1007,7 +1020,7 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_grad_kernel(Scor
   const uint8_t* mask = MASK ? a.r.mask + row * a.r.mask_stride : nullptr;
   T* g = static_cast<T*>(a.grad) + row * a.grad_stride + first;
   Tile<T, NT, NV> tile;
-  tile.load(xr + first, (int)(left < a.sp.chunk ? left : a.sp.chunk));
+  tile.load(xr + first, (int)(left < a.sp.chunk ? left : a.sp.chunk), a.r.big);
   if constexpr (MASK) tile.apply_mask(mask + first);
   int* id = ids[NT == 64 ? threadIdx.x / 64 : 0];
   float* w = ws[NT == 64 ? threadIdx.x / 64 : 0];
@@ -1037,10 +1050,10 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_grad_kernel(Scor
     return __builtin_amdgcn_exp2f(d) * inv_s * (b0 - b1 * fmaxf(d, -200.f));
   };
   if (empty) {
-    write_dense<T, NT, NV>(tile, g, [](float) { return 0.f; });
+    write_dense<T, NT, NV>(tile, g, a.write_past, [](float) { return 0.f; });
     return;
   }
-  write_dense<T, NT, NV>(tile, g, [&](float x) {
+  write_dense<T, NT, NV>(tile, g, a.write_past, [&](float x) {
     const float v = dense(x) * scale;
     return MASK && x == -kInf ? 0.f : v;
   });
@@ -1056,6 +1069,7 @@ struct DistillGradArgs {
   const float *stats, *g_loss;
   void* grad;
   int64_t grad_stride;
+  bool write_past;       // the gradient goes past the cache
 };
 
 template <typename T, int NT, int NV, int LIST>
@@ -1071,13 +1085,13 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_grad_kernel(Di
   const T* x = static_cast<const T*>(a.r.x) + row * a.r.stride + first;
   T* g = static_cast<T*>(a.grad) + row * a.grad_stride + first;
   Tile<T, NT, NV> tile;
-  tile.load(x, (int)(left < a.sp.chunk ? left : a.sp.chunk));
+  tile.load(x, (int)(left < a.sp.chunk ? left : a.sp.chunk), a.r.big);
   int* id = ids[NT == 64 ? threadIdx.x / 64 : 0];
   float* w = ws[NT == 64 ? threadIdx.x / 64 : 0];
   const float* st = a.stats + row * kStats;
   const float m = st[0], inv_s = st[1], mo = st[2], inv_so = st[3], p_o = st[4], log_norm = st[5], q_sum = st[6], rest = st[7];
   if (q_sum == -1.f || inv_s == 0.f) {
-    write_dense<T, NT, NV>(tile, g, [](float) { return 0.f; });
+    write_dense<T, NT, NV>(tile, g, a.write_past, [](float) { return 0.f; });
     return;
   }
   for (int i = group_tid<NT>(); i < a.t.n; i += NT) {
@@ -1090,7 +1104,7 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_grad_kernel(Di
   const float q_all = q_sum + rest;
   // outside the list: p_j q_all - rest e^(z_j - lse_o) = e^(z_j - lse_o) (p_o q_all - rest), p_o the student's bucket
   const float from = tail ? mo : m, a0 = tail ? up * (p_o * q_all - rest) * inv_so : up * q_all * inv_s;
-  write_dense<T, NT, NV>(tile, g, [&](float v) { return a0 * __builtin_amdgcn_exp2f((v - from) * c); });
+  write_dense<T, NT, NV>(tile, g, a.write_past, [&](float v) { return a0 * __builtin_amdgcn_exp2f((v - from) * c); });
   group_sync<NT>();
   write_listed<T, NT>(id, w, a.t.n, x, g, first, tile.n, [&](float v, float q) {
     return up * (__builtin_amdgcn_exp2f((v - m) * c) * inv_s * q_all - q);
@@ -1134,6 +1148,13 @@ __attribute__((format(printf, 2, 3))) int refuse(int code, const char* fmt, ...)
   std::vsnprintf(text, sizeof(text), fmt, ap);
   va_end(ap);
   return fail_without_handle(code, text);
+}
+// Logits that the 256 MB of Infinity Cache do not hold are read past it, and gradients of more than half of it written
+// past it: lines that no one will find there are not written back in the next kernel's time.  us for a loss and its
+// gradient, with / without: 4096 x 49408 bf16 236 / 255, 1024 x 100003 fp32 232 / 266; below, where the backward pass finds
+// the logits in the cache, 62 / 60 (1024 x 49408 bf16) and 93 / 82 (32768 x 1203 fp16): not there.
+bool past_cache(int64_t rows, int64_t vocab, int64_t bytes_each, int64_t limit) {
+  return (double)rows * vocab * bytes_each > limit;
 }
 size_t element_size(int dtype) { return dtype == OAKE_F32 ? 4 : 2; }
 
@@ -1259,7 +1280,8 @@ int oake_token_logprobs(const void* d_logits, int dtype, int64_t rows, int64_t v
   if (int rc = check_scratch(what, d_workspace, workspace_bytes, scratch_bytes(rows, p.sp, top))) return rc;
   float* sums = static_cast<float*>(d_workspace);
   uint64_t* keys = p.sp.parts == 1 ? nullptr : reinterpret_cast<uint64_t*>(sums + rows * p.sp.parts * 4);
-  const ScoreArgs a{{d_logits, rows, vocab, row_stride, d_mask, mask_stride, scale}, p.sp,
+  const ScoreArgs a{{d_logits, rows, vocab, row_stride, d_mask, mask_stride, scale,
+                     past_cache(rows, vocab, element_size(dtype), 256 << 20)}, p.sp,
                     d_targets, index_dtype == OAKE_I64, n_targets, top,
                     d_logprobs, d_lse, d_entropy, d_top_logprobs, d_stats, d_top_indices, sums, keys};
   OAKE_BY_TYPE(dtype, run_score, p, a, (hipStream_t)stream);
@@ -1282,9 +1304,11 @@ int oake_token_logprobs_backward(const void* d_logits, int dtype, int64_t rows, 
   if (!d_stats || (d_grad_logprobs && n_targets && !d_targets) || (d_grad_top && top && !d_top_indices))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
   const Plan p = backward_plan(rows, vocab, dtype, (d_grad_logprobs ? n_targets : 0) + (d_grad_top ? top : 0));
-  const ScoreGradArgs a{{d_logits, rows, vocab, row_stride, d_mask, mask_stride, scale}, p.sp,
+  const ScoreGradArgs a{{d_logits, rows, vocab, row_stride, d_mask, mask_stride, scale,
+                     past_cache(rows, vocab, element_size(dtype), 256 << 20)}, p.sp,
                         d_targets, index_dtype == OAKE_I64, n_targets, top, d_top_indices,
-                        d_stats, d_grad_logprobs, d_grad_lse, d_grad_entropy, d_grad_top, d_grad, grad_stride};
+                        d_stats, d_grad_logprobs, d_grad_lse, d_grad_entropy, d_grad_top, d_grad, grad_stride,
+                        past_cache(rows, vocab, element_size(dtype), 128 << 20)};
   OAKE_BY_TYPE(dtype, run_score_grad, p, a, (hipStream_t)stream);
   return launched(what);
 }
@@ -1300,7 +1324,8 @@ int oake_distill_top_logits(const void* d_logits, int dtype, int64_t rows, int64
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
   const Plan p = forward_plan(rows, vocab, dtype, top);
   if (int rc = check_scratch(what, d_workspace, workspace_bytes, scratch_bytes(rows, p.sp, 0))) return rc;
-  const DistillArgs a{{d_logits, rows, vocab, row_stride, nullptr, 0, scale}, p.sp,
+  const DistillArgs a{{d_logits, rows, vocab, row_stride, nullptr, 0, scale,
+                       past_cache(rows, vocab, element_size(dtype), 256 << 20)}, p.sp,
                       {d_top_indices, d_top_logprobs, index_dtype == OAKE_I64, top, tail != 0}, d_loss, d_stats,
                       static_cast<float*>(d_workspace)};
   OAKE_BY_TYPE(dtype, run_distill, p, a, (hipStream_t)stream);
@@ -1319,9 +1344,11 @@ int oake_distill_top_logits_backward(const void* d_logits, int dtype, int64_t ro
   if (!d_stats || !d_grad_loss || (top && (!d_top_indices || !d_top_logprobs)))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
   const Plan p = backward_plan(rows, vocab, dtype, top);
-  const DistillGradArgs a{{d_logits, rows, vocab, row_stride, nullptr, 0, scale}, p.sp,
+  const DistillGradArgs a{{d_logits, rows, vocab, row_stride, nullptr, 0, scale,
+                       past_cache(rows, vocab, element_size(dtype), 256 << 20)}, p.sp,
                           {d_top_indices, d_top_logprobs, index_dtype == OAKE_I64, top, tail != 0},
-                          d_stats, d_grad_loss, d_grad, grad_stride};
+                          d_stats, d_grad_loss, d_grad, grad_stride,
+                        past_cache(rows, vocab, element_size(dtype), 128 << 20)};
   OAKE_BY_TYPE(dtype, run_distill_grad, p, a, (hipStream_t)stream);
   return launched(what);
 }
