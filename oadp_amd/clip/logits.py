@@ -44,8 +44,8 @@ def _check_logits(logits: torch.Tensor, scale: float) -> None:
         raise TypeError(f'unsupported logits dtype {logits.dtype}')
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f'expected logits [..., vocab >= 1], got {tuple(logits.shape)}')
-    if not 0.0 < scale <= 3.0e38:
-        raise ValueError(f'scale must be positive and finite, got {scale}')
+    if not 0.0 < scale <= 1e38:
+        raise ValueError(f'scale must be positive and at most 1e38, got {scale}')
 
 
 def _check_same_device(logits: torch.Tensor, **others: torch.Tensor | None) -> None:

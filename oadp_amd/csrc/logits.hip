@@ -297,8 +297,8 @@ __device__ __forceinline__ float logp_at(float x, float m, float log_s, float sc
 // A lower bound of the row's top-th largest logit: of the maxima of (at least top) disjoint parts of the row, the top-th
 // largest - that many places reach it.  It is looked for bit by bit in the sort key's upper half by counting over the
 // wave's lanes; the places at or above it go to a list in LDS as keys, and each key's rank is the number of larger ones.
-// 49408 normal logits, 256 parts, top 20: about 21 keys.  A list that overflows (crowded equal values) or a row with
-// NaN (which the maxima pass over) is worked off one alternative at a time instead.
+// 49408 normal logits, 256 parts, top 20: about 21 keys.  Where the list overflows (crowded equal values) or the row has
+// NaN (which the maxima pass over), the top-th key itself is looked for by counting over the row.
 constexpr float kLowest = -3.402823466e38f;
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ float bound_of(uint32_t prefix) {
@@ -418,12 +418,11 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
   constexpr int G = kGroups<NT>, E = kPer<T>, CAP = kListCap<NT>;
   __shared__ __attribute__((aligned(16))) float part_max[NT == 64 ? 1 : kParts];
   __shared__ float tmp_s[NT / 64], tmp_t[NT / 64];
-  __shared__ uint64_t tmp_k[NT / 64];
   constexpr int VECS = kVecCap<NT>;
   __shared__ u32x4_t vecs[G][VECS];
   __shared__ int vec_col[G][VECS], vecs_n[G];
   __shared__ uint64_t list[G][CAP];
-  __shared__ int list_n[G];
+  __shared__ int list_n[G], last_n[G];
   const int64_t index = group_index<NT>();
   if (index >= a.r.rows * a.sp.parts) return;
   const int64_t row = a.sp.parts == 1 ? index : index / a.sp.parts;
@@ -541,12 +540,16 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
     }
   };
   reduce();
-  const uint8_t* mask = MASK ? a.r.mask + row * a.r.mask_stride + first : nullptr;
   if (!ref.fused || (sums.t != sums.t && sums.s == sums.s)) {
-    // logits past what the fused form takes, or -inf among them: again, from memory
+    // logits past what the fused form takes, or -inf among them: again, in the form that takes everything
     if constexpr (NT != 64) __syncthreads();
     sums = Sums();
-    for (int j = t; j < tile.n; j += NT) sums.add(((MASK && !mask[j] ? -kInf : (float)x[j]) - m) * ref.c);
+    tile.pack();
+    tile.each([&](u32x4_t q, int) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) sums.add((elem<T>(q, i) - m) * ref.c);
+    });
+    sums.add((tile.single - m) * ref.c);
     reduce();
   } else {  // relative to m
     sums.s /= ref.one;
@@ -581,42 +584,99 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
     }
   }
   group_sync<NT>();
-  const int n = list_n[g];
-  if (held <= VECS && n <= CAP && sums.s == sums.s) {
-    constexpr int R = NT == 64 ? 2 : 8;  // lanes that count for one key
-    for (int i = t / R; i < n; i += NT / R) {
-      const uint64_t key = list[g][i];
-      int rank = 0;
+  int n = list_n[g];
+  if (held > VECS || n > CAP || sums.s != sums.s) {
+    // Too many equal values at the bound, or NaN: the top-th key itself, by halving over the row, then the last place that
+    // holds an equal one and still counts.  (From memory: the tile's registers are not held for the rare case.)
+    const uint8_t* mask = MASK ? a.r.mask + row * a.r.mask_stride + first : nullptr;
+    const auto key_at = [&](int j) { return order_key(MASK && !mask[j] ? -kInf : (float)x[j]); };
+    const auto count = [&](int places, auto yes) {
+      int c = 0;
 #pragma unroll 8
-      for (int k = t % R; k < n; k += R) rank += list[g][k] > key;
-      rank += __builtin_amdgcn_update_dpp(0, rank, 0xB1, 0xF, 0xF, true);              // quad_perm 1 0 3 2
-      if constexpr (R == 8) {
-        rank += __builtin_amdgcn_update_dpp(0, rank, 0x4E, 0xF, 0xF, true);            // quad_perm 2 3 0 1
-        rank += __builtin_amdgcn_update_dpp(0, rank, 0x141, 0xF, 0xF, true);           // row_half_mirror
+      for (int j = t; j < places; j += NT) c += yes(key_at(j));
+      float sum = wave64_sum((float)c);  // (a chunk has less than 2^24 places)
+      if constexpr (NT != 64) {
+        if (t % 64 == 0) tmp_s[t / 64] = sum;
+        __syncthreads();
+        sum = 0.f;
+        for (int w = 0; w < NT / 64; ++w) sum += tmp_s[w];
+        __syncthreads();
       }
-      if (t % R == 0 && rank < a.top) put(rank, key);
+      return (int)sum;
+    };
+    // keys of one value: those of [v, v + unit)
+    constexpr uint32_t unit = sizeof(T) == 4 ? 1u : __is_same(T, f16_t) ? 1u << 13 : 1u << 16;
+    uint32_t lo = kKeyNegInf + 1, hi = kKeyNan & ~(unit - 1);
+    int above = 0;                       // places with a key of `hi` or more: fewer than top
+    if (sums.s == sums.s) {              // (the bound is right: top places reach it, or it is the lowest number)
+      lo = order_key(bound) & ~(unit - 1);
+      hi = (order_key(m) & ~(unit - 1)) + unit;
+    } else {
+      above = count(tile.n, [&](uint32_t k) { return k >= hi; });
+      if (above >= a.top) lo = hi, above = 0;
     }
-    for (int i = n + t; i < a.top; i += NT) put(i, 0);
-    return;
-  }
-  // (from memory again: the tile's registers are not held for the rare case)
-  uint64_t last = ~0ull;
-  for (int i = 0; i < a.top; ++i) {
-    uint64_t best = 0;
-    for (int j = t; j < tile.n; j += NT) {
-      const uint64_t key = place_key(MASK && !mask[j] ? -kInf : (float)x[j], (uint32_t)(first + j));
-      if (key < last && key > best && (uint32_t)(key >> 32) > kKeyNegInf) best = key;
+    while (lo < hi && hi - lo > unit) {
+      const uint32_t mid = lo + (hi - lo) / 2 / unit * unit;
+      const int c = count(tile.n, [&](uint32_t k) { return k >= mid; });
+      if (c >= a.top) lo = mid;
+      else hi = mid, above = c;
     }
-    best = wave64_max(best);
+    // the waves look through a stretch of the row each for places of the value `lo`; the wave in whose stretch enough of
+    // them come together looks for that place
+    const auto equal = [&](int j) {
+      const uint32_t k = j < tile.n ? key_at(j) : 0;
+      return k > kKeyNegInf && k >= lo && k - lo < unit;
+    };
+    const int wave = NT == 64 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = t % 64;
+    const int stretch = (tile.n + NT - 1) / NT * 64, begin = wave * stretch, need = a.top - above;
+    int mine = 0, before = 0;
+#pragma unroll 8
+    for (int j = begin + lane; j < begin + stretch; j += 64) mine += equal(j);
+    mine = (int)wave64_sum((float)mine);
+    if (t == 0) last_n[g] = tile.n - 1;
     if constexpr (NT != 64) {
-      if (t % 64 == 0) tmp_k[t / 64] = best;
+      if (lane == 0) tmp_s[wave] = (float)mine;
       __syncthreads();
-      for (int w = 0; w < NT / 64; ++w) best = tmp_k[w] > best ? tmp_k[w] : best;
-      __syncthreads();
+      for (int w = 0; w < wave; ++w) before += (int)tmp_s[w];
     }
-    if (t == 0) put(i, best);
-    last = best;  // (0 when nothing is left: nothing is below it)
+    if (before < need && before + mine >= need) {
+      for (int j = begin; before < need; j += 64) {
+        const uint64_t lanes = __ballot(equal(j + lane));
+        const int c = __popcll(lanes);
+        if (before + c >= need) {  // the (need - before)-th of these lanes
+          const int at = __builtin_amdgcn_mbcnt_hi((unsigned)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)lanes, 0));
+          if ((lanes >> lane & 1) && before + at + 1 == need) last_n[g] = j + lane;
+        }
+        before += c;
+      }
+    }
+    group_sync<NT>();
+    const int last = last_n[g];  // places of value `lo` up to here count
+    if (t == 0) list_n[g] = 0;
+    group_sync<NT>();
+    for (int j = t; j < tile.n; j += NT) {
+      const uint32_t k = key_at(j);
+      if (k <= kKeyNegInf || k < lo || (k - lo < unit && j > last)) continue;
+      const int at = atomicAdd(&list_n[g], 1);
+      if (at < CAP) list[g][at] = (uint64_t)k << 32 | (0xFFFFFFFFu - (uint32_t)(first + j));
+    }
+    group_sync<NT>();
+    n = list_n[g] < CAP ? list_n[g] : CAP;
   }
+  constexpr int R = NT == 64 ? 2 : 8;  // lanes that count for one key
+  for (int i = t / R; i < n; i += NT / R) {
+    const uint64_t key = list[g][i];
+    int rank = 0;
+#pragma unroll 8
+    for (int k = t % R; k < n; k += R) rank += list[g][k] > key;
+    rank += __builtin_amdgcn_update_dpp(0, rank, 0xB1, 0xF, 0xF, true);    // quad_perm 1 0 3 2
+    if constexpr (R == 8) {
+      rank += __builtin_amdgcn_update_dpp(0, rank, 0x4E, 0xF, 0xF, true);  // quad_perm 2 3 0 1
+      rank += __builtin_amdgcn_update_dpp(0, rank, 0x141, 0xF, 0xF, true); // row_half_mirror
+    }
+    if (t % R == 0 && rank < a.top) put(rank, key);
+  }
+  for (int i = n + t; i < a.top; i += NT) put(i, 0);
 }
 
 // The chunks of a row joined: sums brought to the largest m, in the chunks' order, and the chunks' lists merged - the rank
@@ -721,7 +781,7 @@ struct Teacher {
 template <int CAP>
 struct TeacherList {  // in LDS
   int id[CAP];
-  float v[CAP];
+  float v[CAP], x[CAP];  // x: the student's logit there
   Teacher t;
 };
 // e^v in 64 bits for what stands in a list: v = n log 2 + r, the series of e^r (|r| <= 0.35: the 12th term is below 1e-14).
@@ -733,16 +793,18 @@ __device__ __forceinline__ double exp64(double v) {
   for (int k = 11; k > 0; --k) p = __builtin_fma(p * (1.0 / k), r, 1.0);
   return v < -200.0 ? 0.0 : __builtin_ldexp(p, (int)n);
 }
-// by one wave (every lane of it), for the group
-template <int CAP>
-__device__ __forceinline__ void teacher_row(const TeacherArgs& a, int64_t row, int64_t vocab, TeacherList<CAP>& s) {
+// By one wave (every lane of it), for the group.  `id`, `v`: the lane's first entry (teacher_entry), fetched before the row
+// was; x (or nullptr): the student's row, whose listed logits are fetched too.
+template <typename T, int CAP>
+__device__ __forceinline__ void teacher_row(const TeacherArgs& a, int64_t row, int64_t vocab, const T* x, int id, float v,
+                                            TeacherList<CAP>& s) {
   const int lane = threadIdx.x % 64;
   float best = -kInf, some = 0.f;
   for (int i = lane; i < a.n; i += 64) {
-    int id;
-    const float v = teacher_entry(a, row, vocab, i, id);
+    if (i != lane) v = teacher_entry(a, row, vocab, i, id);
     s.id[i] = id;
     s.v[i] = v;
+    if (x) s.x[i] = id < 0 ? -kInf : (float)x[id];
     best = fmaxf(best, v);
     if (v != -kInf) some = 1.f;
   }
@@ -783,10 +845,9 @@ __device__ __forceinline__ double log64(float s) {
 }
 // The end of a row, by one group: `m` and `s` are the row's largest logit and sum (tail: of the places outside the list;
 // the listed ones are added here, each place once).
-template <typename T, int NT, int CAP>
+template <int NT, int CAP>
 __device__ __forceinline__ void finish_distill(const DistillArgs& a, int64_t row, const TeacherList<CAP>& te, bool distinct,
                                                float m, float s, float* tmp) {
-  const T* x = static_cast<const T*>(a.r.x) + row * a.r.stride;
   const int t = group_tid<NT>(), n = a.t.n;
   const float scale = a.r.scale, mo = m, so = s;
   float p_o = 1.f;
@@ -794,7 +855,7 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a, int64_t row
     float peak = so == 0.f ? -kInf : mo;
     // (few values: every wave looks at all of them)
     for (int i = t % 64; i < n; i += 64)
-      if (te.id[i] >= 0) peak = fmaxf(peak, (float)x[te.id[i]]);
+      peak = fmaxf(peak, te.x[i]);
     peak = wave64_max(peak);
     m = peak == -kInf ? 0.f : peak;
     s = 0.f;
@@ -802,7 +863,7 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a, int64_t row
       bool first = te.id[i] >= 0;
       if (!distinct)
         for (int k = 0; k < i; ++k) first = first && te.id[k] != te.id[i];
-      if (first) s += __builtin_amdgcn_exp2f(((float)x[te.id[i]] - m) * (scale * kLog2e));
+      if (first) s += __builtin_amdgcn_exp2f((te.x[i] - m) * (scale * kLog2e));
     }
     s = wave64_sum(s);
     p_o = so == 0.f ? 0.f : so * __builtin_amdgcn_exp2f((mo - m) * (scale * kLog2e));
@@ -814,7 +875,7 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a, int64_t row
   for (int i = t; i < n; i += NT) {
     const float v = te.v[i], q = expf(v - te.t.log_norm);
     if (q == 0.f) continue;
-    const float y = te.id[i] < 0 ? v : (float)x[te.id[i]];  // (an id that the vocabulary does not have: v is NaN)
+    const float y = te.id[i] < 0 ? v : te.x[i];  // (an id that the vocabulary does not have: v is NaN)
     const float lost = y == -kInf && s == s ? kInf : (float)((double)v - te.t.log_norm - ((double)y - m) * scale + log_s);
     loss += q * lost;
   }
@@ -853,6 +914,9 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
   const int64_t left = a.r.vocab - first;
   const T* x = static_cast<const T*>(a.r.x) + row * a.r.stride + first;
   const bool whole = a.sp.parts == 1;
+  int id = -1;
+  float v = 0.f;
+  if ((TAIL || whole) && t < 64 && t < a.t.n) v = teacher_entry(a.t, row, a.r.vocab, t, id);
   Tile<T, NT, NV> tile;
   tile.load(x, (int)(left < a.sp.chunk ? left : a.sp.chunk), a.r.big);
   if (t == 0) twice[g] = 0;
@@ -860,8 +924,8 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
     for (int i = t; i < WORDS; i += NT) map[g][i] = 0;
     group_sync<NT>();
   }
-  if (t < 64 && (TAIL || whole)) {
-    teacher_row(a.t, row, a.r.vocab, te[g]);
+  if ((TAIL || whole) && t < 64) {
+    teacher_row(a.t, row, a.r.vocab, whole ? x : nullptr, id, v, te[g]);
     if constexpr (TAIL) {
       for (int i = t; i < a.t.n; i += 64) {
         const int64_t col = te[g].id[i] - first;
@@ -871,53 +935,65 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
       }
     }
   }
-  if constexpr (TAIL) {  // what the list holds is left out
-    group_sync<NT>();
+  // (TAIL: the largest of all places, listed or not - the map is not there yet)
+  const auto largest = [&]() {
+    float m = wave64_max(tile.max());
+    if constexpr (NT != 64) {
+      if (t % 64 == 0) tmp_m[t / 64] = m;
+      __syncthreads();
 #pragma unroll
-    for (int vi = 0; vi < NV; ++vi)
-      if (vi < tile.nv && tile.has_vec(vi)) {
-        const int q = vi * NT + t;
-        const unsigned bits = map[g][q * E / 32] >> q * E % 32 & ((1u << E) - 1);
-        if (bits) {
-#pragma unroll
-          for (int i = 0; i < E; ++i) drop<T>(tile.v[vi], i, bits >> i & 1);
-        }
-      }
-    if (t < 32 && map[g][NT * NV * E / 32] >> t & 1) tile.single = -kInf;
-  }
-  float m = wave64_max(tile.max());
-  if constexpr (NT != 64) {
-    if (t % 64 == 0) tmp_m[t / 64] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < NT / 64; ++w) m = fmaxf(m, tmp_m[w]);
-  } else {
-    group_sync<NT>();
-  }
+      for (int w = 0; w < NT / 64; ++w) m = fmaxf(m, tmp_m[w]);
+    } else {
+      group_sync<NT>();
+    }
+    return m;
+  };
+  float m = largest();
   if ((TAIL || whole) && !te[g].t.some) {  // no teacher: no loss
     if (t == 0 && whole) write_no_teacher(a, row);
     return;
   }
-  const Ref ref(m, a.r.scale * kLog2e);
-  m = ref.m;
-  tile.pack();
-  float s = 0.f;
-  if (ref.fused) {
-    tile.each([&](u32x4_t q, int) {
+  if constexpr (TAIL) {  // what the list holds is left out
+    unsigned bits[NV];
 #pragma unroll
-      for (int i = 0; i < E; ++i) s += __builtin_amdgcn_exp2f(elem_fma<T>(q, i, ref.c, -ref.b));
-    });
-    s += __builtin_amdgcn_exp2f(__builtin_fmaf(tile.single, ref.c, -ref.b));
-  } else {
-    tile.each([&](u32x4_t q, int) {
+    for (int vi = 0; vi < NV; ++vi)  // (the map covers all NV: one wait for all of them)
+      bits[vi] = map[g][(vi * NT + t) * E / 32] >> (vi * NT + t) * E % 32 & ((1u << E) - 1);
 #pragma unroll
-      for (int i = 0; i < E; ++i) s += __builtin_amdgcn_exp2f((elem<T>(q, i) - m) * ref.c);
-    });
-    s += __builtin_amdgcn_exp2f((tile.single - m) * ref.c);
+    for (int vi = 0; vi < NV; ++vi)
+      if (vi < tile.nv && __any(bits[vi] != 0)) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) drop<T>(tile.v[vi], i, bits[vi] >> i & 1);
+      }
+    if (t < 32 && map[g][NT * NV * E / 32] >> t & 1) tile.single = -kInf;
   }
-  s = group_sum<NT>(s, tmp_s) / ref.one;
+  const auto sum = [&]() {
+    const Ref ref(m, a.r.scale * kLog2e);
+    m = ref.m;
+    tile.pack();
+    float s = 0.f;
+    if (ref.fused) {
+      tile.each([&](u32x4_t q, int) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) s += __builtin_amdgcn_exp2f(elem_fma<T>(q, i, ref.c, -ref.b));
+      });
+      s += __builtin_amdgcn_exp2f(__builtin_fmaf(tile.single, ref.c, -ref.b));
+    } else {
+      tile.each([&](u32x4_t q, int) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) s += __builtin_amdgcn_exp2f((elem<T>(q, i) - m) * ref.c);
+      });
+      s += __builtin_amdgcn_exp2f((tile.single - m) * ref.c);
+    }
+    return group_sum<NT>(s, tmp_s) / ref.one;
+  };
+  float s = sum();
+  if (TAIL && s < 1e-30f) {  // the largest is a listed one, far above all others: again, from the largest of those
+    if constexpr (NT != 64) __syncthreads();
+    m = largest();
+    s = sum();
+  }
   if (whole) {
-    finish_distill<T, NT>(a, row, te[g], TAIL && !twice[g], m, s, tmp_l);
+    finish_distill<NT>(a, row, te[g], TAIL && !twice[g], m, s, tmp_l);
   } else if (t == 0) {
     a.part_sums[index * 2] = m;
     a.part_sums[index * 2 + 1] = s;
@@ -931,7 +1007,11 @@ __global__ __launch_bounds__(kThreads) void distill_join_kernel(DistillArgs a) {
   const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
   if (row >= a.r.rows) return;
   const int t = threadIdx.x, parts = a.sp.parts;
-  if (t < 64) teacher_row(a.t, row, a.r.vocab, te);
+  if (t < 64) {
+    int id = -1;
+    const float v = t < a.t.n ? teacher_entry(a.t, row, a.r.vocab, t, id) : 0.f;
+    teacher_row(a.t, row, a.r.vocab, static_cast<const T*>(a.r.x) + row * a.r.stride, id, v, te);
+  }
   __syncthreads();
   if (!te.t.some) {
     if (t == 0) write_no_teacher(a, row);
@@ -946,7 +1026,7 @@ __global__ __launch_bounds__(kThreads) void distill_join_kernel(DistillArgs a) {
   for (int i = t % 64; i < parts; i += 64)
     if (p[i * 2 + 1] != 0.f) s += p[i * 2 + 1] * __builtin_amdgcn_exp2f((p[i * 2] - m) * (a.r.scale * kLog2e));
   s = wave64_sum(s);
-  finish_distill<T, kThreads>(a, row, te, false, m, s, tmp);
+  finish_distill<kThreads>(a, row, te, false, m, s, tmp);
 }
 
 // ---- gradients --------------------------------------------------------------------------------------------------
@@ -1138,7 +1218,10 @@ dim3 grid_of(int64_t blocks) {
   const int64_t x = blocks < 1 << 20 ? blocks : 1 << 20;
   return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
 }
-dim3 grid_of(const Plan& p, int64_t rows) { return grid_of(p.threads == 64 ? (rows + 3) / 4 : rows * p.sp.parts); }
+int64_t blocks_of(const Plan& p, int64_t rows) { return p.threads == 64 ? (rows + 3) / 4 : rows * p.sp.parts; }
+dim3 grid_of(const Plan& p, int64_t rows) { return grid_of(blocks_of(p, rows)); }
+constexpr int64_t kMostBlocks = (int64_t)65535 << 20;
+
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 __attribute__((format(printf, 2, 3))) int refuse(int code, const char* fmt, ...) {
@@ -1164,7 +1247,7 @@ int check_rows(const char* what, const void* x, int dtype, int64_t rows, int64_t
   if (rows < 0 || rows > INT32_MAX || vocab < 1 || vocab > INT32_MAX)
     return refuse(OAKE_ERR_INVALID, "%s: rows must be 0 .. 2^31 - 1 and vocab 1 .. 2^31 - 1", what);
   if (stride < 0) return refuse(OAKE_ERR_INVALID, "%s: a row stride is negative", what);
-  if (!(scale > 0.f) || scale > 3.0e38f) return refuse(OAKE_ERR_INVALID, "%s: scale must be positive and finite", what);
+  if (!(scale > 0.f) || scale > 1e38f) return refuse(OAKE_ERR_INVALID, "%s: scale must be positive and at most 1e38", what);
   if (rows > 0 && !x) return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
   if ((uintptr_t)x % element_size(dtype)) return refuse(OAKE_ERR_INVALID, "%s: the logits are not aligned to their type", what);
   return OAKE_OK;
@@ -1277,6 +1360,7 @@ int oake_token_logprobs(const void* d_logits, int dtype, int64_t rows, int64_t v
   if ((n_targets && (!d_targets || !d_logprobs)) || (top && (!d_top_logprobs || !d_top_indices)))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
   const Plan p = forward_plan(rows, vocab, dtype, 0);
+  if (blocks_of(p, rows) > kMostBlocks) return refuse(OAKE_ERR_INVALID, "%s: too many rows of this length", what);
   if (int rc = check_scratch(what, d_workspace, workspace_bytes, scratch_bytes(rows, p.sp, top))) return rc;
   float* sums = static_cast<float*>(d_workspace);
   uint64_t* keys = p.sp.parts == 1 ? nullptr : reinterpret_cast<uint64_t*>(sums + rows * p.sp.parts * 4);
@@ -1304,6 +1388,7 @@ int oake_token_logprobs_backward(const void* d_logits, int dtype, int64_t rows, 
   if (!d_stats || (d_grad_logprobs && n_targets && !d_targets) || (d_grad_top && top && !d_top_indices))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
   const Plan p = backward_plan(rows, vocab, dtype, (d_grad_logprobs ? n_targets : 0) + (d_grad_top ? top : 0));
+  if (blocks_of(p, rows) > kMostBlocks) return refuse(OAKE_ERR_INVALID, "%s: too many rows of this length", what);
   const ScoreGradArgs a{{d_logits, rows, vocab, row_stride, d_mask, mask_stride, scale,
                      past_cache(rows, vocab, element_size(dtype), 256 << 20)}, p.sp,
                         d_targets, index_dtype == OAKE_I64, n_targets, top, d_top_indices,
@@ -1323,6 +1408,7 @@ int oake_distill_top_logits(const void* d_logits, int dtype, int64_t rows, int64
   if (!d_loss || !d_stats || (top && (!d_top_indices || !d_top_logprobs)))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
   const Plan p = forward_plan(rows, vocab, dtype, top);
+  if (blocks_of(p, rows) > kMostBlocks) return refuse(OAKE_ERR_INVALID, "%s: too many rows of this length", what);
   if (int rc = check_scratch(what, d_workspace, workspace_bytes, scratch_bytes(rows, p.sp, 0))) return rc;
   const DistillArgs a{{d_logits, rows, vocab, row_stride, nullptr, 0, scale,
                        past_cache(rows, vocab, element_size(dtype), 256 << 20)}, p.sp,
@@ -1344,6 +1430,7 @@ int oake_distill_top_logits_backward(const void* d_logits, int dtype, int64_t ro
   if (!d_stats || !d_grad_loss || (top && (!d_top_indices || !d_top_logprobs)))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
   const Plan p = backward_plan(rows, vocab, dtype, top);
+  if (blocks_of(p, rows) > kMostBlocks) return refuse(OAKE_ERR_INVALID, "%s: too many rows of this length", what);
   const DistillGradArgs a{{d_logits, rows, vocab, row_stride, nullptr, 0, scale,
                        past_cache(rows, vocab, element_size(dtype), 256 << 20)}, p.sp,
                           {d_top_indices, d_top_logprobs, index_dtype == OAKE_I64, top, tail != 0},
