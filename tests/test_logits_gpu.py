@@ -137,7 +137,8 @@ def some_targets(rows, vocab, n, seed=0, dtype=torch.int64):
 
 
 # lengths around a wave's, a vector's and a thread block's edges; the text tower's vocabulary; beyond one block's share
-VOCABS = [1, 2, 7, 8, 9, 63, 64, 65, 257, 511, 1203, 2049, 4099, 8191, 16385, 49408, 65537, 131073, 300007]
+VOCABS = [1, 2, 7, 8, 9, 63, 64, 65, 257, 511, 1203, 2048, 2049, 4099, 8192, 8193, 16384, 16385, 32769, 49408, 65536,
+          65543, 131073, 300007]
 
 
 @pytest.mark.parametrize('dtype', TYPES)
@@ -229,6 +230,81 @@ def test_many_equal_logits(cuda, vocab, dtype):
     x[2, 100:228] = 50
     x[3, ::vocab // 130] = 45
     Score(x, None, 128).check(token_logprobs(x, top=128))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab', [700, 2000, 9000, 49408, 140001])
+def test_crowded_rows(cuda, vocab, dtype):
+    """More places at the border than any list holds: equal values in a stretch, in the whole row, at its end, NaN among them,
+    and the same among masked places."""
+    g = torch.Generator(device='cuda').manual_seed(vocab)
+    x = logits_of(8, vocab, dtype, spread=1.0)
+    x[0] = -3.5                                                    # all equal and negative
+    x[1, vocab // 3:] = 9                                          # ... behind a third of the row
+    x[2, vocab // 2:] = torch.finfo(dtype).max
+    x[3, :40] = 30                                                 # fewer than asked for above, the rest equal
+    x[3, 40:] = -2
+    x[4, torch.randperm(vocab, generator=g, device='cuda')[:vocab // 2]] = float('nan')
+    x[5, :50] = float('nan')                                       # fewer NaN than asked for, then equal ones
+    x[5, 50:] = 1
+    x[6, :] = -INF
+    x[6, vocab - 300:] = 0.125
+    x[7] = torch.arange(vocab, device='cuda').to(dtype) * 1e-3     # (16 bits: steps of many places)
+    mask = torch.rand(8, vocab, generator=g, device='cuda') < 0.6
+    for top in (1, 64, 128):
+        Score(x, None, top).check(token_logprobs(x, top=top))
+        Score(x, None, top, mask=mask).check(token_logprobs(x, top=top, mask=mask))
+
+
+@pytest.mark.parametrize('vocab', [300, 6000, 60000])
+def test_sizes_of_values(cuda, vocab):
+    """Logits whose scaled size leaves no digits for their differences, that differ by many powers of ten, or that run
+    through zero: log probabilities of d = scale * (x - max x), alternatives in the order of x."""
+    x = logits_of(7, vocab, torch.float32)
+    x[0] += 1e6                                                    # differences of whole steps of 1 / 16
+    x[1] *= 1e20
+    x[2] = x[2].abs() * 10 ** (torch.arange(vocab, device='cuda') % 30 - 15.0)
+    x[3] = -x[3].abs() * 10 ** (torch.arange(vocab, device='cuda') % 30 - 15.0)
+    x[4] *= 1e-30
+    x[5, ::3] = -3e38
+    x[6] = -torch.rand(vocab, generator=torch.Generator(device='cuda').manual_seed(1), device='cuda') * 1e-6
+    for scale in (1.0, 1e-3, 50.0):
+        ours, ref = token_logprobs(x, top=100, scale=scale), Score(x, None, 100, scale=scale)
+        assert torch.equal(ours.top_indices, ref.top_indices)
+        # (z = scale * x in 64 bits has all digits of the fp32 product that lse is)
+        close(ours.entropy, ref.h, ref.tol_h[:, 0] + 1e-9)
+        close(ours.top_logprobs, ref.top_logprobs, ref.tol_top + 4 * E * ref.top_logprobs.abs())
+
+
+def test_lists_of_many_chunks(cuda):
+    """A vocabulary of 37 chunks with the longest lists: more keys than the join holds at once."""
+    x = logits_of(2, 1200007, torch.float32)
+    t = some_targets(2, 1200007, 3)
+    Score(x, t, 128).check(token_logprobs(x, t, top=128))
+    ids, v = a_teacher(2, 1200007, 128)
+    leaf = x.requires_grad_()
+    up = torch.rand(2, device=cuda)
+    loss = distill_top_logits(leaf, ids, v, tail=True)
+    grad, = torch.autograd.grad([loss], [leaf], [up])
+    Distill(leaf, ids, v, 1.0, True).check(loss, grad, up)
+
+
+def test_large_logits_past_the_cache(cuda):
+    """Logits of 300 MB and their gradient, read and written past the cache, row by row what a small call gives."""
+    x = logits_of(1600, 49153, torch.float32).requires_grad_()
+    t = some_targets(1600, 49153, 1)
+    w = torch.rand(1600, 1, generator=torch.Generator().manual_seed(0)).to(cuda)
+    out = token_logprobs(x, t, top=4)
+    grad, = torch.autograd.grad([out.logprobs], [x], [w])
+    ids, v = out.top_indices, out.top_logprobs.detach()
+    g2, = torch.autograd.grad([distill_top_logits(x, ids, v, scale=0.5, tail=True)], [x], [w[:, 0]])
+    for rows in (slice(0, 3), slice(797, 800), slice(1597, 1600)):
+        s = x.detach()[rows].requires_grad_()
+        small = token_logprobs(s, t[rows], top=4)
+        assert all(torch.equal(a[rows], b) for a, b in zip(out, small))
+        assert torch.equal(grad[rows], torch.autograd.grad([small.logprobs], [s], [w[rows]])[0])
+        loss = distill_top_logits(s, ids[rows], v[rows], scale=0.5, tail=True)
+        assert torch.equal(g2[rows], torch.autograd.grad([loss], [s], [w[rows, 0]])[0])
 
 
 def test_clip_scale(cuda):
