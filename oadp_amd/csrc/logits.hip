@@ -349,7 +349,7 @@ constexpr int kParts = 256;  // maxima of a workgroup's parts
 template <int NT>
 constexpr int kListCap = NT == 64 ? 256 : 1024;  // keys
 template <int NT>
-constexpr int kVecCap = NT == 64 ? 96 : 512;     // vectors that hold some
+constexpr int kVecCap = NT == 64 ? 144 : 512;    // vectors that hold some
 
 // ---- token_logprobs -----------------------------------------------------------------------------------------
 struct ScoreArgs {
@@ -1193,11 +1193,15 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_grad_kernel(Di
 
 // ---- launches -----------------------------------------------------------------------------------------------------
 // Who works on a row: a wave where its registers hold the row (four rows a workgroup, no barriers), a workgroup of 256
-// threads, or of 1024 - beyond that the row is cut into equal chunks, which a second launch joins.
+// threads, or of 512 - beyond that the row is cut into equal chunks, which a second launch joins.
+// Rows of 2049 .. 4096 places go to a wave with twice the vectors where there are enough of them to fill the device at its
+// half occupancy and few alternatives to look for (wave / workgroup, us: 32768 x 2500 bf16, 20 alternatives 54 / 96;
+// 2400 x 2500 8.1 / 11.3; 1024 x 4000 7.4 / 7.0; 8192 x 2500, 100 alternatives 99 / 51; 2400 x 4000 fp32, 20 12.9 / 12.7).
 constexpr int kBlockVecs = 8, kLongVecs = 16, kGradVecs = 4;
 constexpr int kWaveList = 64;  // entries of a list that a wave's share of the LDS holds
 struct Plan {
   int threads;  // 64, 256, 512
+  bool twice;   // a wave with 2 * kWaveVecs vectors a lane
   Split sp;
 };
 int64_t capacity(int threads, int vecs, int dtype) { return (int64_t)threads * vecs * (dtype == OAKE_F32 ? 4 : 8); }
@@ -1205,14 +1209,17 @@ Split split(int64_t vocab, int64_t most) {  // equal chunks of at most `most` pl
   const int64_t parts = (vocab + most - 1) / most, chunk = ((vocab + parts - 1) / parts + 7) / 8 * 8;
   return {chunk, (int)((vocab + chunk - 1) / chunk)};
 }
-Plan forward_plan(int64_t rows, int64_t vocab, int dtype, int list) {
-  if (vocab <= kWavePlaces && list <= kWaveList) return {64, {vocab, 1}};
-  if (vocab <= capacity(256, kBlockVecs, dtype)) return {256, {vocab, 1}};
-  return {512, split(vocab, capacity(512, kLongVecs, dtype))};
+Plan forward_plan(int64_t rows, int64_t vocab, int dtype, int top, int list) {
+  if (list <= kWaveList) {
+    if (vocab <= kWavePlaces) return {64, false, {vocab, 1}};
+    if (vocab <= 2 * kWavePlaces && rows >= 2048 && top <= 32) return {64, true, {vocab, 1}};
+  }
+  if (vocab <= capacity(256, kBlockVecs, dtype)) return {256, false, {vocab, 1}};
+  return {512, false, split(vocab, capacity(512, kLongVecs, dtype))};
 }
 Plan backward_plan(int64_t rows, int64_t vocab, int dtype, int list) {
-  if (vocab <= kWavePlaces && list <= kWaveList) return {64, {vocab, 1}};
-  return {256, split(vocab, capacity(256, kGradVecs, dtype))};
+  if (vocab <= kWavePlaces && list <= kWaveList) return {64, false, {vocab, 1}};
+  return {256, false, split(vocab, capacity(256, kGradVecs, dtype))};
 }
 dim3 grid_of(int64_t blocks) {
   const int64_t x = blocks < 1 << 20 ? blocks : 1 << 20;
@@ -1278,7 +1285,8 @@ void run_score(const Plan& p, const ScoreArgs& a, hipStream_t s) {
 #define OAKE_SCORE(NT, NV)                                                                    \
   if (a.r.mask) score_kernel<T, NT, NV, true><<<grid, kBlock<NT>, 0, s>>>(a);        \
   else score_kernel<T, NT, NV, false><<<grid, kBlock<NT>, 0, s>>>(a)
-  if (p.threads == 64) { OAKE_SCORE(64, kWaveVecs<T>); }
+  if (p.twice) { OAKE_SCORE(64, 2 * kWaveVecs<T>); }
+  else if (p.threads == 64) { OAKE_SCORE(64, kWaveVecs<T>); }
   else if (p.threads == 256) { OAKE_SCORE(256, kBlockVecs); }
   else { OAKE_SCORE(512, kLongVecs); }
 #undef OAKE_SCORE
@@ -1301,7 +1309,8 @@ void run_distill(const Plan& p, const DistillArgs& a, hipStream_t s) {
 #define OAKE_DISTILL(NT, NV, LIST)                                                                  \
   if (a.t.tail) distill_kernel<T, NT, NV, true, LIST><<<grid, kBlock<NT>, 0, s>>>(a);      \
   else distill_kernel<T, NT, NV, false, LIST><<<grid, kBlock<NT>, 0, s>>>(a)
-  if (p.threads == 64) { OAKE_DISTILL(64, kWaveVecs<T>, kWaveList); }
+  if (p.twice) { OAKE_DISTILL(64, 2 * kWaveVecs<T>, kWaveList); }
+  else if (p.threads == 64) { OAKE_DISTILL(64, kWaveVecs<T>, kWaveList); }
   else if (p.threads == 256) { OAKE_DISTILL(256, kBlockVecs, kMaxList); }
   else { OAKE_DISTILL(512, kLongVecs, kMaxList); }
 #undef OAKE_DISTILL
@@ -1343,7 +1352,7 @@ int oake_logits_workspace(int64_t rows, int64_t vocab, int dtype, int top, size_
   if (!bytes) return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
   if (int rc = check_rows(what, bytes, dtype, rows, vocab, vocab, 1.f)) return rc;
   if (top < 0 || top > kMaxTop) return refuse(OAKE_ERR_INVALID, "%s: top must be 0 .. %d", what, kMaxTop);
-  *bytes = scratch_bytes(rows, forward_plan(rows, vocab, dtype, 0).sp, top);
+  *bytes = scratch_bytes(rows, forward_plan(rows, vocab, dtype, top, 0).sp, top);
   return OAKE_OK;
 }
 
@@ -1359,7 +1368,7 @@ int oake_token_logprobs(const void* d_logits, int dtype, int64_t rows, int64_t v
   if (rows == 0) return OAKE_OK;
   if ((n_targets && (!d_targets || !d_logprobs)) || (top && (!d_top_logprobs || !d_top_indices)))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
-  const Plan p = forward_plan(rows, vocab, dtype, 0);
+  const Plan p = forward_plan(rows, vocab, dtype, top, 0);
   if (blocks_of(p, rows) > kMostBlocks) return refuse(OAKE_ERR_INVALID, "%s: too many rows of this length", what);
   if (int rc = check_scratch(what, d_workspace, workspace_bytes, scratch_bytes(rows, p.sp, top))) return rc;
   float* sums = static_cast<float*>(d_workspace);
@@ -1407,7 +1416,7 @@ int oake_distill_top_logits(const void* d_logits, int dtype, int64_t rows, int64
   if (rows == 0) return OAKE_OK;
   if (!d_loss || !d_stats || (top && (!d_top_indices || !d_top_logprobs)))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
-  const Plan p = forward_plan(rows, vocab, dtype, top);
+  const Plan p = forward_plan(rows, vocab, dtype, 0, top);
   if (blocks_of(p, rows) > kMostBlocks) return refuse(OAKE_ERR_INVALID, "%s: too many rows of this length", what);
   if (int rc = check_scratch(what, d_workspace, workspace_bytes, scratch_bytes(rows, p.sp, 0))) return rc;
   const DistillArgs a{{d_logits, rows, vocab, row_stride, nullptr, 0, scale,

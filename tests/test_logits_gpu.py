@@ -153,7 +153,8 @@ def test_scores_over_lengths(cuda, vocab, dtype):
 
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('rows, vocab, top', [(1, 65, 5), (1, 1203, 20), (1, 49408, 5), (1, 151936, 128), (2, 49408, 64),
-                                              (17, 20001, 10), (300, 65, 8), (700, 1203, 33), (1300, 4097, 7), (600, 9999, 1)])
+                                              (17, 20001, 10), (300, 65, 8), (700, 1203, 33), (1300, 4097, 7), (600, 9999, 1), (2500, 2049, 20),
+                                              (2500, 4096, 32), (2050, 3001, 128), (400, 1999, 128), (400, 1203, 100)])
 def test_scores_over_rows(cuda, rows, vocab, top, dtype):
     x = logits_of(rows, vocab, dtype, seed=3)
     t = some_targets(rows, vocab, 1)
@@ -233,7 +234,7 @@ def test_many_equal_logits(cuda, vocab, dtype):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
-@pytest.mark.parametrize('vocab', [700, 2000, 9000, 49408, 140001])
+@pytest.mark.parametrize('vocab', [700, 2000, 3500, 9000, 49408, 140001])
 def test_crowded_rows(cuda, vocab, dtype):
     """More places at the border than any list holds: equal values in a stretch, in the whole row, at its end, NaN among them,
     and the same among masked places."""
@@ -251,9 +252,12 @@ def test_crowded_rows(cuda, vocab, dtype):
     x[6, vocab - 300:] = 0.125
     x[7] = torch.arange(vocab, device='cuda').to(dtype) * 1e-3     # (16 bits: steps of many places)
     mask = torch.rand(8, vocab, generator=g, device='cuda') < 0.6
-    for top in (1, 64, 128):
+    for top in (1, 20, 64, 128):
         Score(x, None, top).check(token_logprobs(x, top=top))
         Score(x, None, top, mask=mask).check(token_logprobs(x, top=top, mask=mask))
+    if vocab < 4096:  # as many rows as another share of the work takes
+        x, mask = x.repeat(256, 1), mask.repeat(256, 1)
+        Score(x, None, 20, mask=mask).check(token_logprobs(x, top=20, mask=mask))
 
 
 @pytest.mark.parametrize('vocab', [300, 6000, 60000])
@@ -476,7 +480,7 @@ def a_teacher(rows, vocab, k, seed=0, index=torch.int64):
 @pytest.mark.parametrize('tail', [False, True])
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('rows, vocab, k', [(3, 1, 1), (4, 2, 1), (5, 9, 4), (5, 9, 9), (5, 9, 12), (300, 65, 8), (3, 511, 1),
-                                            (40, 1203, 20), (7, 1203, 300), (6, 5001, 64), (3, 49408, 128), (2, 140001, 1000)])
+                                            (40, 1203, 20), (7, 1203, 300), (6, 5001, 64), (3, 49408, 128), (2, 140001, 1000), (2100, 2301, 20)])
 def test_distillation(cuda, rows, vocab, k, dtype, tail):
     x = logits_of(rows, vocab, dtype, seed=8).requires_grad_()
     ids, v = a_teacher(rows, vocab, k, index=torch.int32 if k % 2 else torch.int64)
