@@ -178,6 +178,15 @@ __device__ __forceinline__ uint64_t wave64_max(uint64_t v) {
   }
   return v;
 }
+// over the two / eight neighbouring lanes that count for one key
+__device__ __forceinline__ int sum2(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, true);  // quad_perm 1 0 3 2
+}
+__device__ __forceinline__ int sum8(int v) {
+  v = sum2(v);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, true);           // quad_perm 2 3 0 1
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, true);  // row_half_mirror
+}
 template <int NT, typename V>
 __device__ __forceinline__ V group_sum(V v, V* tmp) {  // tmp: NT / 64 values, free when the call begins
   v = wave64_sum(v);
@@ -669,22 +678,21 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
     int rank = 0;
 #pragma unroll 8
     for (int k = t % R; k < n; k += R) rank += list[g][k] > key;
-    rank += __builtin_amdgcn_update_dpp(0, rank, 0xB1, 0xF, 0xF, true);    // quad_perm 1 0 3 2
-    if constexpr (R == 8) {
-      rank += __builtin_amdgcn_update_dpp(0, rank, 0x4E, 0xF, 0xF, true);  // quad_perm 2 3 0 1
-      rank += __builtin_amdgcn_update_dpp(0, rank, 0x141, 0xF, 0xF, true); // row_half_mirror
-    }
+    rank = R == 8 ? sum8(rank) : sum2(rank);
     if (t % R == 0 && rank < a.top) put(rank, key);
   }
   for (int i = n + t; i < a.top; i += NT) put(i, 0);
 }
 
-// The chunks of a row joined: sums brought to the largest m, in the chunks' order, and the chunks' lists merged - the rank
-// of a key is its place in its own list plus, for each other list, how many keys of that are larger (a binary search).
-constexpr int kJoinCap = 4096;  // keys that are looked at in LDS (32 KB); more stay in memory
+// The chunks of a row joined: sums brought to the largest m, in the chunks' order, and the chunks' lists.  Of every list its
+// ceil(top / chunks)-th key: at least `top` keys reach the least of these, and each of those is ranked by the number of larger
+// ones.  Where they are too many for the LDS (equal values in most lists), a key's rank is its place in its own list plus,
+// for each other list, how many keys of that are larger (a binary search).
+constexpr int kJoinCap = 2048;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
   __shared__ uint64_t list[kJoinCap];
+  __shared__ int list_n;
   const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
   if (row >= a.r.rows) return;
   const int t = threadIdx.x, parts = a.sp.parts, top = a.top;
@@ -715,46 +723,57 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
 
   const int64_t total = (int64_t)parts * top;
   const uint64_t* all = a.part_keys + row * total;
-  int some = 0;  // alternatives of the row that this thread has seen: the rest of the answer is filled up
   const int share = (top + parts - 1) / parts - 1;
-  const auto merge = [&](const uint64_t* keys) {
-    // of every list its share'th key: at least `top` keys reach the least of these
-    uint64_t bound = ~0ull;
-    for (int p = 0; p < parts; ++p) {
-      const uint64_t k = keys[(int64_t)p * top + share];
-      bound = k < bound ? k : bound;
+  if (t == 0) list_n = 0;
+  uint64_t bound = ~0ull;  // (by every wave for itself; 0: a list has fewer keys, and all of them are looked at)
+  for (int p = t % 64; p < parts; p += 64) {
+    const uint64_t k = all[(int64_t)p * top + share];
+    bound = k < bound ? k : bound;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint64_t k = __shfl_xor(bound, o, 64);
+    bound = k < bound ? k : bound;
+  }
+  if (bound == 0) bound = 1;
+  __syncthreads();
+  for (int64_t i = t; i < total; i += kThreads) {
+    const uint64_t key = all[i];
+    if (key < bound) continue;
+    const int at = atomicAdd(&list_n, 1);
+    if (at < kJoinCap) list[at] = key;
+  }
+  __syncthreads();
+  const int n = list_n;
+  if (n <= kJoinCap) {
+    for (int i = t / 8; i < n; i += kThreads / 8) {  // eight lanes count for one key
+      const uint64_t key = list[i];
+      int rank = 0;
+#pragma unroll 8
+      for (int k = t % 8; k < n; k += 8) rank += list[k] > key;
+      rank = sum8(rank);
+      if (t % 8 == 0 && rank < top) write_top(a, row, st, rank, key);
     }
+  } else {
     for (int64_t i = t; i < total; i += kThreads) {
-      const uint64_t key = keys[i];
-      some += key != 0;
-      if (key == 0 || key < bound) continue;
+      const uint64_t key = all[i];
+      if (key < bound) continue;
       const int own = (int)(i / top);
       int64_t rank = i - (int64_t)own * top;
-#pragma unroll 8
-      for (int p = 0; p < parts; ++p) {
-        const uint64_t* other = keys + (int64_t)p * top;
+      for (int p = 0; p < parts && rank < top; ++p) {
+        if (p == own) continue;
+        const uint64_t* other = all + (int64_t)p * top;
         int lo = 0;  // keys of the other list before `lo` are larger
-#pragma unroll
         for (int step = kMaxTop; step > 0; step /= 2) {
           const int at = lo + step < top ? lo + step : top;
           lo = other[at - 1] > key ? at : lo;
         }
-        rank += p == own ? 0 : lo;
+        rank += lo;
       }
       if (rank < top) write_top(a, row, st, (int)rank, key);
     }
-  };
-  if (total <= kJoinCap) {
-    for (int i = t; i < (int)total; i += kThreads) list[i] = all[i];
-    __syncthreads();
-    merge(list);
-  } else {
-    merge(all);
   }
-  __shared__ float tmp[kThreads / 64];
-  const float found = group_sum<kThreads>((float)some, tmp);
-  for (int i = t; i < top; i += kThreads)
-    if (i >= found) write_top(a, row, st, i, 0);
+  for (int i = n + t; i < top; i += kThreads) write_top(a, row, st, i, 0);
 }
 
 // ---- the teacher's list of one row ----------------------------------------------------------------------------

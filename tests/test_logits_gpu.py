@@ -282,12 +282,13 @@ def test_sizes_of_values(cuda, vocab):
 
 def test_lists_of_many_chunks(cuda):
     """A vocabulary of 37 chunks with the longest lists: more keys than the join holds at once."""
-    x = logits_of(2, 1200007, torch.float32)
-    t = some_targets(2, 1200007, 3)
+    x = logits_of(3, 1200007, torch.float32)
+    x[1] = 1.5  # every chunk's list is full of equal values
+    t = some_targets(3, 1200007, 3)
     Score(x, t, 128).check(token_logprobs(x, t, top=128))
-    ids, v = a_teacher(2, 1200007, 128)
+    ids, v = a_teacher(3, 1200007, 128)
     leaf = x.requires_grad_()
-    up = torch.rand(2, device=cuda)
+    up = torch.rand(3, device=cuda)
     loss = distill_top_logits(leaf, ids, v, tail=True)
     grad, = torch.autograd.grad([loss], [leaf], [up])
     Distill(leaf, ids, v, 1.0, True).check(loss, grad, up)
