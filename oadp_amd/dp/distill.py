@@ -9,23 +9,32 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
-from ..clip.logits import distill_top_logits, label_logits, token_logprobs
+from ..clip.logits import MAX_TOP, distill_top_logits, label_logits, token_logprobs
 
 
 class TopLogitsDistillation:
     """``loss(student_logits, embeddings)`` -> KL(teacher || student) per crop, differentiable in the student's logits.
 
-    ``labels`` [n, embed]: label embeddings on the student's device.  ``scale``: CLIP's logit scale; ``temperature`` T
-    divides the teacher's and the student's logits alike, and the loss is multiplied by T^2 so that its gradient keeps its
-    size.  ``tail``: what the list leaves out counts as one more outcome (``distill_top_logits``).  ``mask`` (bool [n]):
-    the labels that are taught - the others are left out of the teacher's distribution."""
+    ``labels`` [n, embed]: label embeddings on the student's device.  ``top`` (1 .. 128; at most n are there): entries of
+    the teacher's list.  ``scale``: CLIP's logit scale; ``temperature`` T divides the teacher's and the student's logits
+    alike, and the loss is multiplied by T^2 so that its gradient keeps its size.  ``tail``: what the list leaves out counts
+    as one more outcome (``distill_top_logits``).  ``mask`` (bool [n]): the labels that are taught - the others are left out
+    of the teacher's distribution."""
 
     def __init__(self, labels: torch.Tensor, *, top: int = 32, scale: float = 100.0, temperature: float = 1.0,
                  tail: bool = True, mask: torch.Tensor | None = None) -> None:
-        if labels.dim() != 2:
-            raise ValueError(f'expected label embeddings [n, embed], got {tuple(labels.shape)}')
-        if not temperature > 0:
-            raise ValueError(f'temperature must be positive, got {temperature}')
+        if labels.dim() != 2 or labels.shape[0] < 1:
+            raise ValueError(f'expected label embeddings [n >= 1, embed], got {tuple(labels.shape)}')
+        if not 1 <= int(top) <= MAX_TOP:
+            raise ValueError(f'top must be 1 .. {MAX_TOP}, got {top}')
+        if not 0 < temperature < float('inf'):
+            raise ValueError(f'temperature must be positive and finite, got {temperature}')
+        if not 0 < scale / temperature <= 1e38:
+            raise ValueError(f'scale / temperature must be positive and at most 1e38, got {scale} / {temperature}')
+        if mask is not None and mask.dtype != torch.bool:
+            raise TypeError(f'mask must be bool, got {mask.dtype}')
+        if mask is not None and mask.shape != labels.shape[:1]:
+            raise ValueError(f'expected a mask {(labels.shape[0],)}, got {tuple(mask.shape)}')
         self.labels = F.normalize(labels.detach().float(), dim=-1)
         self.mask = mask
         self.top = min(int(top), labels.shape[0])

@@ -106,3 +106,14 @@ def test_c_refusals(lib):
     for args in [(-1, 100, _lib.OAKE_F16, 5), (4, 0, _lib.OAKE_F16, 5), (4, 100, _lib.OAKE_U8, 5), (4, 100, _lib.OAKE_F16, 129)]:
         assert lib.oake_logits_workspace(*args, C.byref(n)) == _lib.OAKE_ERR_INVALID
     assert lib.oake_logits_workspace(4, 100, _lib.OAKE_F16, 5, None) == _lib.OAKE_ERR_INVALID
+
+
+@pytest.mark.parametrize('options', [dict(top=0), dict(top=-3), dict(top=129), dict(scale=0.0), dict(scale=float('nan')),
+                                     dict(temperature=float('nan')), dict(temperature=float('inf')),
+                                     dict(mask=torch.ones(4, dtype=torch.bool)), dict(mask=torch.ones(5))])
+def test_distillation_refuses_before_the_first_batch(options):
+    with pytest.raises((ValueError, TypeError)):
+        TopLogitsDistillation(torch.zeros(5, 8), **options)
+    with pytest.raises(ValueError):
+        TopLogitsDistillation(torch.zeros(0, 8))
+    assert TopLogitsDistillation(torch.zeros(5, 8), top=128).top == 5
