@@ -9,7 +9,9 @@
 
 The arithmetic runs in hand-written gfx950 kernels behind the C ABI (``oake_token_logprobs``, ``oake_distill_top_logits``
 and their backward passes, include/oake_hip.h, which states every special case); tensors must live on the GPU.  Calls use
-the current stream of the logits' device, whichever device is current, and can be captured into a graph.
+the current stream of the logits' device, whichever device is current, and can be captured into a graph.  (A backward pass
+is captured with leaves made for the capture, on its stream and with no other graph of theirs alive: torch accumulates a
+leaf's gradient on the stream its first graph was built on, and a capture does not take that.)
 """
 from __future__ import annotations
 
@@ -292,4 +294,5 @@ def label_logits(embeddings: torch.Tensor, labels: torch.Tensor) -> torch.Tensor
     ensemble of ``oadp_amd.prompts.vild``); both are normalised here."""
     if labels.dim() != 2 or embeddings.shape[-1] != labels.shape[1]:
         raise ValueError(f'embeddings {tuple(embeddings.shape)} and labels {tuple(labels.shape)} do not match')
-    return F.normalize(embeddings.float(), dim=-1) @ F.normalize(labels.float(), dim=-1).t()
+    with torch.autocast(embeddings.device.type, enabled=False):  # (a cosine of 16 bits times CLIP's scale is off by 0.2)
+        return F.normalize(embeddings.float(), dim=-1) @ F.normalize(labels.float(), dim=-1).t()

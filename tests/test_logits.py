@@ -108,6 +108,16 @@ def test_c_refusals(lib):
     assert lib.oake_logits_workspace(4, 100, _lib.OAKE_F16, 5, None) == _lib.OAKE_ERR_INVALID
 
 
+def test_label_logits_under_autocast():
+    """The cosines stay fp32: rounded to 16 bits and times CLIP's scale they would be off by 0.2 and more."""
+    e, labels = torch.randn(4, 16, generator=torch.Generator().manual_seed(0)), torch.eye(16)[:5] + 0.1
+    want = label_logits(e, labels)
+    with torch.autocast('cpu', dtype=torch.bfloat16):
+        got = label_logits(e, labels)
+        assert torch.is_autocast_enabled('cpu')
+    assert got.dtype == torch.float32 and torch.equal(got, want)
+
+
 @pytest.mark.parametrize('options', [dict(top=0), dict(top=-3), dict(top=129), dict(scale=0.0), dict(scale=float('nan')),
                                      dict(temperature=float('nan')), dict(temperature=float('inf')),
                                      dict(mask=torch.ones(4, dtype=torch.bool)), dict(mask=torch.ones(5))])
