@@ -2,6 +2,12 @@
 // partition sum and the top alternatives; a student's distillation loss against a teacher's top logits; the gradients
 // of both.  The C entry points are at the end of the file (include/oake_hip.h states what they compute).
 //
+// Each forward kernel reads the logits once and keeps them in registers for its second look (the largest first, then the
+// sums relative to it), each backward kernel reads them once and writes the gradient: memory is the bound.  A copy of
+// 2 x 0.54 GB reaches 5.3 TB/s on this card, 2 x 2.1 GB 4.9; a 16-bit logit at that rate leaves about 15 lane operations
+// of time, so the forward kernels' instructions per logit count as well (VALU busy 0.72 in the first example below).
+// Times at the kernels are of the kernel alone.
+//
 // A row of `vocab` logits x (fp32, fp16 or bf16) and a positive scale give z = scale * x and p = softmax(z).  Everything
 // is kept relative to the row's largest logit m: d = scale * (x - m) <= 0, S = sum e^d, so that log p = d - log S keeps
 // its digits where it is small, whatever the size of m (lse = scale * m + log S is rounded once, at the end).  All of it
@@ -36,7 +42,6 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 __device__ __forceinline__ uint64_t place_key(float x, uint32_t j) {
   return (uint64_t)order_key(x) << 32 | (0xFFFFFFFFu - j);
 }
-
 
 struct Rows {  // rows of logits and what of them is allowed
   const void* x;
@@ -202,7 +207,9 @@ __device__ __forceinline__ V group_sum(V v, V* tmp) {  // tmp: NT / 64 values, f
 // ---- a chunk of a row in the registers of a group ----------------------------------------------------------------
 // The places are NV vectors of 16 bytes a thread, vector v of thread t being number v * NT + t of the chunk's, and, behind
 // the last whole vector, one single value each of the first threads.  Rows of odd length put the vectors at any element's
-// address.
+// address.  (fp32 rows lose nothing by that; 16-bit ones do, 2048 x 131071 bf16 122 us against 95 for 131072.  Whole words
+// put together in registers took 170; vectors from the first aligned place on 139, and a row's sums would depend on where
+// it lies.)
 template <typename T, int NT, int NV>
 struct Tile {
   u32x4_t v[NV];
@@ -303,11 +310,11 @@ __device__ __forceinline__ float logp_at(float x, float m, float log_s, float sc
 }
 
 // ---- the top alternatives -------------------------------------------------------------------------------------
-// A lower bound of the row's top-th largest logit: of the maxima of (at least top) disjoint parts of the row, the top-th
-// largest - that many places reach it.  It is looked for bit by bit in the sort key's upper half by counting over the
-// wave's lanes; the places at or above it go to a list in LDS as keys, and each key's rank is the number of larger ones.
-// 49408 normal logits, 256 parts, top 20: about 21 keys.  Where the list overflows (crowded equal values) or the row has
-// NaN (which the maxima pass over), the top-th key itself is looked for by counting over the row.
+// A lower bound of the row's top-th largest logit: of the maxima of (at least top) disjoint parts of the row, about the
+// top-th largest - that many places reach it.  It is looked for by counting over the wave's lanes.  In the pass of the sums
+// the vectors that hold a place at or above it go to LDS as they are, their places there become keys, and each key's rank is
+// the number of larger ones.  49408 normal logits, 256 parts, top 20: about 21 keys.  Where a list overflows (crowded equal
+// values) or the row has NaN (which the maxima pass over), the top-th key itself is looked for by counting over the row.
 constexpr float kLowest = -3.402823466e38f;
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ float bound_of(uint32_t prefix) {
@@ -422,6 +429,12 @@ __device__ __forceinline__ void write_top(const ScoreArgs& a, int64_t row, const
   a.top_logprobs[row * a.top + rank] = some ? (x - st.m) * a.r.scale - st.log_s : -kInf;
 }
 
+// One row, or one chunk of it, a group.  Bound by memory: 4096 x 49408 bf16 with 20 alternatives 84 us = 4.8 TB/s (78
+// without alternatives, 107 with 100), 2048 x 131071 130 us = 4.1 (an odd row length, and two chunks a row).  Rows that a
+// wave holds are bound by its instructions, most of them the alternatives': 65536 x 1203 fp16, top 20, 62 us = 2.5 TB/s
+// with the VALU busy for 0.87 of it; small calls by the launch (300 x 65 5.7 us, 1728 x 1203 with a mask 8.3, 1 x 49408 6.9).
+// Rows off the common way: a mask for each row 150 us at 4096 x 49408, -inf among the logits 120, all equal 775, NaN in every
+// row 1745.
 template <typename T, int NT, int NV, bool MASK>
 __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs a) {
   constexpr int G = kGroups<NT>, E = kPer<T>, CAP = kListCap<NT>;
@@ -458,9 +471,19 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
   if constexpr (NT == 64) {
     m = wave64_max(mine);
     if (a.top) {
-      // parts: the lanes' own places where enough of them have any; else each place for itself
+      // Parts: the lanes' own places, or the vectors, where there are twice as many as are wanted; else each place for itself
+      // (exact, but eight times the counting.  Vectors / places, us: 16384 x 2000 bf16, 100 alternatives, 64 / 91; 8192 x 1203
+      // fp16, 50 21 / 38, 100 - 1.5 vectors for each - 49 / 47, 128 86 / 54: too many keys to rank).
       if (a.top <= 32 && tile.nvec >= 2 * a.top) {
         bound = bound_by_bits(a.top, [&](float v) { return __popcll(__ballot(mine >= v)); });
+      } else if (tile.nvec >= 2 * a.top) {
+        bound = bound_by_bits(a.top, [&](float v) {
+          int n = 0;
+#pragma unroll
+          for (int vi = 0; vi < NV; ++vi)
+            if (vi < tile.nv) n += __popcll(__ballot(tile.has_vec(vi) && vmax[vi] >= v));
+          return n;
+        });
       } else {
         bound = bound_by_bits(a.top, [&](float v) {
           int n = __popcll(__ballot(tile.single >= v));
@@ -687,7 +710,8 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
 // The chunks of a row joined: sums brought to the largest m, in the chunks' order, and the chunks' lists.  Of every list its
 // ceil(top / chunks)-th key: at least `top` keys reach the least of these, and each of those is ranked by the number of larger
 // ones.  Where they are too many for the LDS (equal values in most lists), a key's rank is its place in its own list plus,
-// for each other list, how many keys of that are larger (a binary search).
+// for each other list, how many keys of that are larger (a binary search).  Bound by its chain of dependent steps: 16 rows of
+// seven chunks with 100 alternatives 8.9 us, 2048 rows of two with 64 9.5.
 constexpr int kJoinCap = 2048;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
@@ -804,7 +828,7 @@ struct TeacherList {  // in LDS
   Teacher t;
 };
 // e^v in 64 bits for what stands in a list: v = n log 2 + r, the series of e^r (|r| <= 0.35: the 12th term is below 1e-14).
-// (The library's exp would take the workgroup of 1024 past 64 registers a thread, and so to one a CU.)
+// (The library's exp is what would set the kernel's registers.)
 __device__ __forceinline__ double exp64(double v) {
   const double n = __builtin_rint(v * 1.4426950408889634), r = __builtin_fma(n, -0.69314718055994531, v);
   double p = 1.0;
@@ -915,8 +939,12 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a, int64_t row
   }
 }
 
-// Places of a chunk by the bits of a map in LDS: vectors first (a vector's bits are a byte, or half of one), then the
-// single places.
+// One row, or one chunk of it, a group; the teacher's list is read beside the row by the group's first wave.  TAIL: the sum
+// over the places outside the list is what is kept (1 - sum of the listed p would lose it to rounding), the listed places
+// being known by the bits of a map in LDS: vectors first (a vector's bits are a byte, or half of one), then the single ones.
+// Bound by memory: 4096 x 49408 bf16, 64 entries, 81 us = 5.0 TB/s; 1024 x 100003 fp32 with the bucket, in four chunks a row,
+// 69 + 8.6 for the join = 5.3; 2400 x 1203 fp16 8.5, 300 x 65 5.2: there the list's exponentials and logarithms in 64 bits,
+// one after the other.
 template <typename T, int NT, int NV, bool TAIL, int LIST>
 __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(DistillArgs a) {
   constexpr int G = kGroups<NT>, E = kPer<T>, WORDS = TAIL ? NT * NV * E / 32 + 1 : 1;
@@ -1019,6 +1047,7 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
   }
 }
 
+// The chunks of a row joined, as above: of the sums, and the loss from the list (whose logits are read here).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void distill_join_kernel(DistillArgs a) {
   __shared__ TeacherList<kMaxList> te;
@@ -1104,6 +1133,9 @@ struct ScoreGradArgs {
   bool write_past;       // the gradient goes past the cache
 };
 
+// One row a wave, or a chunk of 256 threads with four vectors each: what it needs beside the logits is in the forward pass's
+// stats, so chunks need no join, and short ones keep more of them in flight.  Bound by memory: 2048 x 49408 fp16 65.5 us =
+// 6.2 TB/s read and written (the forward pass has left part of the logits in the Infinity Cache), 777 x 1203 fp32 6.4 us.
 template <typename T, int NT, int NV, bool MASK, int LIST>
 __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_grad_kernel(ScoreGradArgs a) {
   constexpr int G = kGroups<NT>;
@@ -1171,6 +1203,7 @@ struct DistillGradArgs {
   bool write_past;       // the gradient goes past the cache
 };
 
+// As above.  4096 x 49408 bf16 151 us = 5.4 TB/s, 1024 x 100003 fp32 144 = 5.7, 2400 x 1203 fp16 7.1, 300 x 65 4.4.
 template <typename T, int NT, int NV, int LIST>
 __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_grad_kernel(DistillGradArgs a) {
   constexpr int G = kGroups<NT>;
@@ -1211,11 +1244,16 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_grad_kernel(Di
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------
-// Who works on a row: a wave where its registers hold the row (four rows a workgroup, no barriers), a workgroup of 256
-// threads, or of 512 - beyond that the row is cut into equal chunks, which a second launch joins.
+// Who works on a row, by its length alone: a wave where its registers hold the row (four rows a workgroup, no barriers; by
+// wave / 256 threads, us: 300 x 65 fp32, 5 alternatives 4.7 / 9.7, 16384 x 2000 fp16, 20 23 / 63, 65536 x 1203 62 / 233,
+// its gradient 62 / 100), a workgroup of 256 threads with 8 vectors each, or of 512 with 16 (256 / 512: 2400 x 4500 bf16
+// 11.9 / 26, 8192 x 16000 49 / 93) - beyond that the row is cut into equal chunks, which a second launch joins.  The chunks
+// are as long as they can be, few rows or many: a quarter as long with 256 threads, the join has four times the lists (a
+// quarter / whole, us with the join: 16 x 200003 fp32, 100 alternatives 23 / 19, 20 14.6 / 11.9, 1 x 262143 bf16 11.9 /
+// 12.8, 32 x 131071 bf16 12.3 / 15.6).  Gradients need no join and take 256 threads with 4 vectors (2 or 8: within 5 %).
 // Rows of 2049 .. 4096 places go to a wave with twice the vectors where there are enough of them to fill the device at its
 // half occupancy and few alternatives to look for (wave / workgroup, us: 32768 x 2500 bf16, 20 alternatives 54 / 96;
-// 2400 x 2500 8.1 / 11.3; 1024 x 4000 7.4 / 7.0; 8192 x 2500, 100 alternatives 99 / 51; 2400 x 4000 fp32, 20 12.9 / 12.7).
+// 2400 x 2500 8.1 / 11.3; 1024 x 4000 7.4 / 7.0; 8192 x 4000 fp32, 100 alternatives 61 / 52; 2400 x 4000 fp32, 20 12.9 / 12.7).
 constexpr int kBlockVecs = 8, kLongVecs = 16, kGradVecs = 4;
 constexpr int kWaveList = 64;  // entries of a list that a wave's share of the LDS holds
 struct Plan {
@@ -1247,7 +1285,6 @@ dim3 grid_of(int64_t blocks) {
 int64_t blocks_of(const Plan& p, int64_t rows) { return p.threads == 64 ? (rows + 3) / 4 : rows * p.sp.parts; }
 dim3 grid_of(const Plan& p, int64_t rows) { return grid_of(blocks_of(p, rows)); }
 constexpr int64_t kMostBlocks = (int64_t)65535 << 20;
-
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 __attribute__((format(printf, 2, 3))) int refuse(int code, const char* fmt, ...) {
@@ -1296,7 +1333,6 @@ int launched(const char* what) {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? OAKE_OK : refuse(OAKE_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
-
 
 template <typename T>
 void run_score(const Plan& p, const ScoreArgs& a, hipStream_t s) {
@@ -1418,7 +1454,7 @@ int oake_token_logprobs_backward(const void* d_logits, int dtype, int64_t rows, 
   const Plan p = backward_plan(rows, vocab, dtype, (d_grad_logprobs ? n_targets : 0) + (d_grad_top ? top : 0));
   if (blocks_of(p, rows) > kMostBlocks) return refuse(OAKE_ERR_INVALID, "%s: too many rows of this length", what);
   const ScoreGradArgs a{{d_logits, rows, vocab, row_stride, d_mask, mask_stride, scale,
-                     past_cache(rows, vocab, element_size(dtype), 256 << 20)}, p.sp,
+                         past_cache(rows, vocab, element_size(dtype), 256 << 20)}, p.sp,
                         d_targets, index_dtype == OAKE_I64, n_targets, top, d_top_indices,
                         d_stats, d_grad_logprobs, d_grad_lse, d_grad_entropy, d_grad_top, d_grad, grad_stride,
                         past_cache(rows, vocab, element_size(dtype), 128 << 20)};
@@ -1460,10 +1496,10 @@ int oake_distill_top_logits_backward(const void* d_logits, int dtype, int64_t ro
   const Plan p = backward_plan(rows, vocab, dtype, top);
   if (blocks_of(p, rows) > kMostBlocks) return refuse(OAKE_ERR_INVALID, "%s: too many rows of this length", what);
   const DistillGradArgs a{{d_logits, rows, vocab, row_stride, nullptr, 0, scale,
-                       past_cache(rows, vocab, element_size(dtype), 256 << 20)}, p.sp,
+                           past_cache(rows, vocab, element_size(dtype), 256 << 20)}, p.sp,
                           {d_top_indices, d_top_logprobs, index_dtype == OAKE_I64, top, tail != 0},
                           d_stats, d_grad_loss, d_grad, grad_stride,
-                        past_cache(rows, vocab, element_size(dtype), 128 << 20)};
+                          past_cache(rows, vocab, element_size(dtype), 128 << 20)};
   OAKE_BY_TYPE(dtype, run_distill_grad, p, a, (hipStream_t)stream);
   return launched(what);
 }
