@@ -207,9 +207,11 @@ __device__ __forceinline__ V group_sum(V v, V* tmp) {  // tmp: NT / 64 values, f
 // ---- a chunk of a row in the registers of a group ----------------------------------------------------------------
 // The places are NV vectors of 16 bytes a thread, vector v of thread t being number v * NT + t of the chunk's, and, behind
 // the last whole vector, one single value each of the first threads.  Rows of odd length put the vectors at any element's
-// address.  (fp32 rows lose nothing by that; 16-bit ones do, 2048 x 131071 bf16 122 us against 95 for 131072.  Whole words
-// put together in registers took 170; vectors from the first aligned place on 139, and a row's sums would depend on where
-// it lies.)
+// address: fp32 vectors lose nothing by that, 16-bit ones that begin inside a word do.  Where the loads are the bound
+// (workgroups of 512) those come from the word before and move down by one element, whose place the next lane's first word
+// fills - by one load for all vectors of a wave where that is another wave's, or none (shifted / as they lie, us: 2048 x 131071
+// bf16, 64 alternatives 130 / 147, 4096 x 49409, 20 98 / 107; 49408 87); where instructions or stores are, they are loaded as
+// they lie (65536 x 1203 fp16 69 / 67, the gradient of 65536 x 1203 69 / 64, of 2048 x 49409 70 / 67).
 template <typename T, int NT, int NV>
 struct Tile {
   u32x4_t v[NV];
@@ -222,12 +224,21 @@ struct Tile {
   __device__ __forceinline__ bool has_single() const { return group_tid<NT>() < n - nvec * kPer<T>; }
   __device__ __forceinline__ bool has_vec(int vi) const { return vi * NT + group_tid<NT>() < nvec; }
 
+  static constexpr bool kShift = NT == 512 && sizeof(T) == 2;
+
   __device__ __forceinline__ void load(const T* x, int count, bool past_cache) {
     n = count;
     nvec = n / kPer<T>;
     const int wave = NT == 64 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x) & ~63;
     nv = nvec > wave ? (nvec - wave + NT - 1) / NT : 0;
-    const u32x4_any* p = reinterpret_cast<const u32x4_any*>(x) + group_tid<NT>();
+    const bool shift = kShift && (reinterpret_cast<uintptr_t>(x) & 2);
+    unsigned behind = 0;  // lane vi: the last element of the wave's vectors number vi
+    if (shift) {
+      const int lane = threadIdx.x % 64, end = lane * NT + wave + 63;
+      if (lane < nv) behind = reinterpret_cast<const unsigned short*>(x)[(end < nvec ? end : nvec - 1) * kPer<T> + kPer<T> - 1];
+    }
+    // (the element before an odd one is the other half of its word, and so in the same allocation)
+    const u32x4_any* p = reinterpret_cast<const u32x4_any*>(x - (shift ? 1 : 0)) + group_tid<NT>();
     if (past_cache) {
 #pragma unroll
       for (int vi = 0; vi < NV; ++vi)
@@ -242,6 +253,21 @@ struct Tile {
     }
     single = -kInf;
     if (has_single()) single = (float)x[single_col()];
+    if (shift) {
+#pragma unroll
+      for (int vi = 0; vi < NV; ++vi)
+        if (vi < nv) {
+          const unsigned last = __builtin_amdgcn_readlane(behind, vi);
+          u32x4_t q = v[vi];
+          q[0] = has_vec(vi) ? q[0] : last;
+          const unsigned next = __builtin_amdgcn_update_dpp((int)last, (int)q[0], 0x130, 0xF, 0xF, false);  // wave_shl:1
+          q[0] = __builtin_amdgcn_alignbit(q[1], q[0], 16);
+          q[1] = __builtin_amdgcn_alignbit(q[2], q[1], 16);
+          q[2] = __builtin_amdgcn_alignbit(q[3], q[2], 16);
+          q[3] = __builtin_amdgcn_alignbit(next, q[3], 16);
+          v[vi] = q;
+        }
+    }
   }
   // what the mask (of the chunk's first place on) leaves out becomes -inf
   __device__ __forceinline__ void apply_mask(const uint8_t* mask) {
@@ -430,7 +456,7 @@ __device__ __forceinline__ void write_top(const ScoreArgs& a, int64_t row, const
 }
 
 // One row, or one chunk of it, a group.  Bound by memory: 4096 x 49408 bf16 with 20 alternatives 84 us = 4.8 TB/s (78
-// without alternatives, 107 with 100), 2048 x 131071 130 us = 4.1 (an odd row length, and two chunks a row).  Rows that a
+// without alternatives, 107 with 100), 2048 x 131071 in two chunks a row 127 with the join = 4.2.  Rows that a
 // wave holds are bound by its instructions, most of them the alternatives': 65536 x 1203 fp16, top 20, 62 us = 2.5 TB/s
 // with the VALU busy for 0.87 of it; small calls by the launch (300 x 65 5.7 us, 1728 x 1203 with a mask 8.3, 1 x 49408 6.9).
 // Rows off the common way: a mask for each row 150 us at 4096 x 49408, -inf among the logits 120, all equal 775, NaN in every

@@ -724,3 +724,23 @@ def test_teacher_and_student(cuda, n, top, tail, temperature):
         ref = Distill(same.detach().reshape(80, n), ids.reshape(80, -1), v.reshape(80, -1), 1 / temperature, tail)
         assert (learnt.reshape(80, 1).abs() <= temperature ** 2 * (ref.tol + 8 * E)).all()
         assert grad.abs().max() <= temperature * (2 * ref.off_p.max() + 200 * E)
+
+
+@pytest.mark.parametrize('dtype', (torch.float16, torch.bfloat16, torch.float32))
+@pytest.mark.parametrize('vocab', (1, 7, 9, 2056, 8192, 16385, 16392, 33288, 49407, 65536, 65537, 131071, 200003))
+def test_rows_at_any_element(cuda, dtype, vocab):
+    """The same rows from an even and from an odd element on, NaN before, between and behind them: the same bits."""
+    x = logits_of(3, vocab, dtype)
+    outs = []
+    for offset, gap in ((0, 8 - vocab % 8), (1, 1 + vocab % 2), (3, 8 - vocab % 8), (2, 1 + vocab % 2), (0, 1 - vocab % 2 + 1)):
+        buf = torch.full((offset + 3 * (vocab + gap) + 8,), float('nan'), dtype=dtype, device=cuda)
+        rows = torch.as_strided(buf, (3, vocab), (vocab + gap, 1), offset)
+        rows.copy_(x)
+        a = token_logprobs(rows, torch.tensor([0, vocab - 1, vocab // 2], device=cuda), top=min(vocab, 24))
+        losses = [distill_top_logits(rows, a.top_indices, a.top_logprobs, scale=0.7, tail=tail) for tail in (False, True)]
+        leaf = rows.detach().requires_grad_()
+        grad, = torch.autograd.grad(token_logprobs(leaf).entropy.sum(), [leaf])
+        outs.append([*a, *losses, grad])
+    assert not outs[0][2].isnan().any()
+    for other in outs[1:]:
+        assert all(torch.equal(w, o) for w, o in zip(outs[0], other))
