@@ -968,7 +968,7 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a, int64_t row
 // One row, or one chunk of it, a group; the teacher's list is read beside the row by the group's first wave.  TAIL: the sum
 // over the places outside the list is what is kept (1 - sum of the listed p would lose it to rounding), the listed places
 // being known by the bits of a map in LDS: vectors first (a vector's bits are a byte, or half of one), then the single ones.
-// Bound by memory: 4096 x 49408 bf16, 64 entries, 81 us = 5.0 TB/s; 1024 x 100003 fp32 with the bucket, in four chunks a row,
+// Bound by memory: 4096 x 49408 bf16, 64 entries, 83 us = 4.9 TB/s; 1024 x 100003 fp32 with the bucket, in four chunks a row,
 // 69 + 8.6 for the join = 5.3; 2400 x 1203 fp16 8.5, 300 x 65 5.2: there the list's exponentials and logarithms in 64 bits,
 // one after the other.
 template <typename T, int NT, int NV, bool TAIL, int LIST>
@@ -1160,8 +1160,8 @@ struct ScoreGradArgs {
 };
 
 // One row a wave, or a chunk of 256 threads with four vectors each: what it needs beside the logits is in the forward pass's
-// stats, so chunks need no join, and short ones keep more of them in flight.  Bound by memory: 2048 x 49408 fp16 65.5 us =
-// 6.2 TB/s read and written (the forward pass has left part of the logits in the Infinity Cache), 777 x 1203 fp32 6.4 us.
+// stats, so chunks need no join, and short ones keep more of them in flight.  Bound by memory: 2048 x 49408 fp16 67 us =
+// 6.0 TB/s read and written (the forward pass has left part of the logits in the Infinity Cache), 777 x 1203 fp32 6.4 us.
 template <typename T, int NT, int NV, bool MASK, int LIST>
 __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_grad_kernel(ScoreGradArgs a) {
   constexpr int G = kGroups<NT>;
