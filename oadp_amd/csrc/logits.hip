@@ -499,8 +499,11 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
     if (a.top) {
       // Parts: the lanes' own places, or the vectors, where there are twice as many as are wanted; else each place for itself
       // (exact, but eight times the counting.  Vectors / places, us: 16384 x 2000 bf16, 100 alternatives, 64 / 91; 8192 x 1203
-      // fp16, 50 21 / 38, 100 - 1.5 vectors for each - 49 / 47, 128 86 / 54: too many keys to rank).
-      if (a.top <= 32 && tile.nvec >= 2 * a.top) {
+      // fp16, 50 21 / 38, 100 - 1.5 vectors for each - 49 / 47, 128 86 / 54: too many keys to rank).  So few places that ranking
+      // all of them takes less than that: no bound (19200 x 65 fp16, 5 alternatives 27 / 35, x 17 15 / 35; 121 places 50 / 36).
+      if (tile.n <= 96 && tile.nvec < 2 * a.top) {
+        bound = kLowest;
+      } else if (a.top <= 32 && tile.nvec >= 2 * a.top) {
         bound = bound_by_bits(a.top, [&](float v) { return __popcll(__ballot(mine >= v)); });
       } else if (tile.nvec >= 2 * a.top) {
         bound = bound_by_bits(a.top, [&](float v) {
