@@ -1,4 +1,4 @@
-"""Consumer side of the OAKE feature files (SURVEY.md §8f rank 4): access layers + ``LoadCLIPFeatures``, and
+"""Consumer side of the OAKE feature files: access layers + ``LoadCLIPFeatures``, and
 the loss a detector's classifier takes from them: ``TopLogitsDistillation``."""
 from .distill import TopLogitsDistillation
 from .features import LoadCLIPFeatures, PackAccessLayer, PthAccessLayer, build_access_layer, pack
