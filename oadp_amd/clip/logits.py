@@ -41,6 +41,12 @@ class TokenLogprobs(NamedTuple):
     top_indices: torch.Tensor | None    # [..., top], -1 where there are fewer alternatives
 
 
+def _check_scale(scale: float | torch.Tensor) -> float:
+    if isinstance(scale, torch.Tensor) and scale.requires_grad and torch.is_grad_enabled():
+        raise ValueError('scale gets no gradient: detach() it, or multiply the logits by a learnt scale')
+    return float(scale)
+
+
 def _check_logits(logits: torch.Tensor, scale: float) -> None:
     if logits.dtype not in _DTYPES:
         raise TypeError(f'unsupported logits dtype {logits.dtype}')
@@ -183,9 +189,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     (NaN and inf included) is without effect and its gradient is 0.  A row with nothing allowed: lse -inf, entropy 0,
     log probabilities -inf, gradient 0.
 
-    Differentiable once in ``logits`` through logprobs, entropy, lse and top_logprobs (a log probability of -inf is a
-    constant)."""
-    scale, top = float(scale), int(top)
+    Differentiable once in ``logits`` (not in ``scale``: multiply the logits by a learnt one) through logprobs, entropy,
+    lse and top_logprobs (a log probability of -inf is a constant)."""
+    scale, top = _check_scale(scale), int(top)
     _check_logits(logits, scale)
     if not 0 <= top <= MAX_TOP:
         raise ValueError(f'top must be 0 .. {MAX_TOP}, got {top}')
@@ -260,8 +266,8 @@ def distill_top_logits(logits: torch.Tensor, top_indices: torch.Tensor, top_logp
     from moving its mass out of (or into) the list.  Temperature T: ``scale = 1 / T`` here and for the teacher's call,
     and T^2 times the loss to keep the gradient's size.
 
-    Differentiable once in ``logits``; the teacher gets no gradient."""
-    scale, tail = float(scale), bool(tail)
+    Differentiable once in ``logits``; the teacher and ``scale`` get no gradient."""
+    scale, tail = _check_scale(scale), bool(tail)
     _check_logits(logits, scale)
     if top_indices.dtype not in _INDEX:
         raise TypeError(f'top_indices must be int32 or int64, got {top_indices.dtype}')

@@ -127,3 +127,16 @@ def test_distillation_refuses_before_the_first_batch(options):
     with pytest.raises(ValueError):
         TopLogitsDistillation(torch.zeros(0, 8))
     assert TopLogitsDistillation(torch.zeros(5, 8), top=128).top == 5
+
+
+def test_a_learnt_scale_is_refused():
+    """A scale that wants a gradient would silently get none; without one, or without grad mode, it is a number."""
+    learnt = torch.nn.Parameter(torch.tensor(2.0))
+    for call in (lambda s: token_logprobs(X, scale=s), lambda s: distill_top_logits(X, IDS, LP, scale=s)):
+        for scale in (learnt, learnt.exp()):
+            with pytest.raises(ValueError, match='scale'):
+                call(scale)
+        with pytest.raises(RuntimeError, match='GPU'):  # past the checks of arguments
+            call(learnt.detach())
+        with torch.no_grad(), pytest.raises(RuntimeError, match='GPU'):
+            call(learnt)
