@@ -744,3 +744,26 @@ def test_rows_at_any_element(cuda, dtype, vocab):
     assert not outs[0][2].isnan().any()
     for other in outs[1:]:
         assert all(torch.equal(w, o) for w, o in zip(outs[0], other))
+
+
+@pytest.mark.parametrize('rows, vocab', [(5, 1), (7, 65), (6, 1203), (3, 49409)])
+def test_saved_tensors_that_come_back_packed(cuda, rows, vocab):
+    """Logits and a mask with rows of their own strides, moved to the host and back between the two passes."""
+    base = logits_of(rows, vocab + 13, torch.float16)
+    allowed = torch.rand(rows, vocab + 70, device=cuda) < 0.7
+    allowed[:, 11] = True
+    x, mask, t = base[:, 5:5 + vocab], allowed[:, 11:11 + vocab], some_targets(rows, vocab, 2)
+    up = torch.randn(rows, device=cuda)
+
+    def step():
+        leaf = x.detach().requires_grad_()
+        a = token_logprobs(leaf, t, top=3, mask=mask)
+        loss = distill_top_logits(leaf, a.top_indices, a.top_logprobs.detach(), scale=0.5, tail=True)
+        return torch.autograd.grad([a.logprobs, a.entropy, a.top_logprobs, loss], [leaf],
+                                   [up[:, None].expand(rows, 2), up, up[:, None].expand(rows, 3), up])[0]
+
+    want = step()
+    with torch.autograd.graph.save_on_cpu():
+        got = step()
+    assert torch.equal(got, want)
+    assert vocab == 1 or want.abs().sum() > 0
