@@ -847,7 +847,8 @@ __device__ __forceinline__ float teacher_entry(const TeacherArgs& a, int64_t row
 // q = e^(v - log_norm): the softmax of the row's entries, or (tail) e^v as they are and a bucket for what is left of 1,
 // a difference from 1 that is taken in 64 bits
 struct Teacher {
-  float log_norm, q_sum, q_rest;
+  double log_norm;
+  float q_sum, q_rest;
   bool some;  // there is an entry at all
 };
 template <int CAP>
@@ -864,6 +865,13 @@ __device__ __forceinline__ double exp64(double v) {
 #pragma unroll
   for (int k = 11; k > 0; --k) p = __builtin_fma(p * (1.0 / k), r, 1.0);
   return v < -200.0 ? 0.0 : __builtin_ldexp(p, (int)n);
+}
+// log s in 64 bits: that of s in fp32, and one step of Newton's on e^y = s (which squares its error of 2^-24).
+__device__ __forceinline__ double log64(double s) {
+  if (s == 0) return -__builtin_inf();
+  const int n = __builtin_amdgcn_frexp_exp(s);
+  const double part = __builtin_ldexp(s, -n), y = logf((float)part);
+  return y + (part * exp64(-y) - 1.0) + n * 0.69314718055994531;
 }
 // By one wave (every lane of it), for the group.  `id`, `v`: the lane's first entry (teacher_entry), fetched before the row
 // was; x (or nullptr): the student's row, whose listed logits are fetched too.
@@ -887,9 +895,9 @@ __device__ __forceinline__ void teacher_row(const TeacherArgs& a, int64_t row, i
   double sum = 0;
   for (int i = lane; i < a.n; i += 64) sum += exp64((double)s.v[i] - best);
   sum = wave64_sum(sum);
-  const float log_norm = a.tail || sum == 0 ? best : best + logf((float)sum);
+  const double log_norm = a.tail || sum == 0 ? best : best + log64(sum);
   float q_sum = 0.f;
-  for (int i = lane; i < a.n; i += 64) q_sum += expf(s.v[i] - log_norm);
+  for (int i = lane; i < a.n; i += 64) q_sum += expf((float)(s.v[i] - log_norm));
   q_sum = wave64_sum(q_sum);
   if (lane == 0) s.t = {log_norm, q_sum, a.tail ? (float)(sum > 1 ? 0 : 1 - sum) : 0.f, some != 0.f};
 }
@@ -905,47 +913,45 @@ struct DistillArgs {
 // What the backward pass needs of a row: m, 1 / S (0: the student has nothing); the same outside the list; the student's
 // probability there; the teacher's log_norm, q_sum (-1: no entry) and bucket
 constexpr int kStats = 8;
+constexpr int kExactPlaces = 64;  // rows of so many are summed in 64 bits (few classes: a loss of 1e-4 and less is ordinary)
 __device__ __forceinline__ void write_no_teacher(const DistillArgs& a, int64_t row) {
   a.loss[row] = 0.f;
   a.stats[row * kStats + 6] = -1.f;
 }
 
-// log s to about 2^-25 whatever its size, for the few places whose log p and log q are nearly equal
-__device__ __forceinline__ double log64(float s) {
-  const int n = __builtin_amdgcn_frexp_expf(s);
-  return (double)logf(__builtin_ldexpf(s, -n)) + n * 0.69314718055994531;
-}
 // The end of a row, by one group: `m` and `s` are the row's largest logit and sum (tail: of the places outside the list;
-// the listed ones are added here, each place once).
+// the listed ones are added here, each place once).  Where teacher and student nearly agree the loss is a difference of equal
+// logarithms: those, the list's sums and (short rows) all sums are taken in 64 bits.
 template <int NT, int CAP>
 __device__ __forceinline__ void finish_distill(const DistillArgs& a, int64_t row, const TeacherList<CAP>& te, bool distinct,
-                                               float m, float s, float* tmp) {
+                                               float m, double s, float* tmp) {
   const int t = group_tid<NT>(), n = a.t.n;
-  const float scale = a.r.scale, mo = m, so = s;
+  const float scale = a.r.scale, mo = m;
+  const double so = s;
   float p_o = 1.f;
   if (a.t.tail) {
-    float peak = so == 0.f ? -kInf : mo;
+    float peak = so == 0 ? -kInf : mo;
     // (few values: every wave looks at all of them)
     for (int i = t % 64; i < n; i += 64)
       peak = fmaxf(peak, te.x[i]);
     peak = wave64_max(peak);
     m = peak == -kInf ? 0.f : peak;
-    s = 0.f;
+    s = 0;
     for (int i = t % 64; i < n; i += 64) {
       bool first = te.id[i] >= 0;
       if (!distinct)
         for (int k = 0; k < i; ++k) first = first && te.id[k] != te.id[i];
-      if (first) s += __builtin_amdgcn_exp2f((te.x[i] - m) * (scale * kLog2e));
+      if (first) s += exp64(((double)te.x[i] - m) * scale);
     }
     s = wave64_sum(s);
-    p_o = so == 0.f ? 0.f : so * __builtin_amdgcn_exp2f((mo - m) * (scale * kLog2e));
-    s += p_o;
-    p_o /= s;
+    const double outside = so == 0 ? 0 : so * exp64(((double)mo - m) * scale);
+    s += outside;
+    p_o = (float)(outside / s);
   }
   const double log_s = log64(s);
   float loss = 0.f;
   for (int i = t; i < n; i += NT) {
-    const float v = te.v[i], q = expf(v - te.t.log_norm);
+    const float v = te.v[i], q = expf((float)(v - te.t.log_norm));
     if (q == 0.f) continue;
     const float y = te.id[i] < 0 ? v : te.x[i];  // (an id that the vocabulary does not have: v is NaN)
     const float lost = y == -kInf && s == s ? kInf : (float)((double)v - te.t.log_norm - ((double)y - m) * scale + log_s);
@@ -953,16 +959,16 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a, int64_t row
   }
   loss = group_sum<NT>(loss, tmp);
   if (t == 0) {
-    const float rest = !a.t.tail || so == 0.f ? 0.f : te.t.q_rest;
+    const float rest = !a.t.tail || so == 0 ? 0.f : te.t.q_rest;
     if (rest != 0.f) loss += rest * (float)(log64(rest) - ((double)mo - m) * scale - log64(so) + log_s);
     a.loss[row] = loss;
     float* st = a.stats + row * kStats;
     st[0] = m;
-    st[1] = s == 0.f ? 0.f : 1.f / s;
+    st[1] = s == 0 ? 0.f : (float)(1 / s);
     st[2] = mo;
-    st[3] = so == 0.f ? 0.f : 1.f / so;
+    st[3] = so == 0 ? 0.f : (float)(1 / so);
     st[4] = p_o;
-    st[5] = te.t.log_norm;
+    st[5] = (float)te.t.log_norm;
     st[6] = te.t.q_sum;
     st[7] = rest;
   }
@@ -1042,10 +1048,21 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
       }
     if (t < 32 && map[g][NT * NV * E / 32] >> t & 1) tile.single = -kInf;
   }
-  const auto sum = [&]() {
+  const auto sum = [&]() -> double {
     const Ref ref(m, a.r.scale * kLog2e);
     m = ref.m;
     tile.pack();
+    if constexpr (NT == 64) {
+      if (tile.n <= kExactPlaces) {
+        const auto e = [&](float v) { return exp64(((double)v - m) * a.r.scale); };
+        double s = e(tile.single);
+        tile.each([&](u32x4_t q, int) {
+#pragma unroll
+          for (int i = 0; i < E; ++i) s += e(elem<T>(q, i));
+        });
+        return wave64_sum(s);
+      }
+    }
     float s = 0.f;
     if (ref.fused) {
       tile.each([&](u32x4_t q, int) {
@@ -1062,8 +1079,8 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
     }
     return group_sum<NT>(s, tmp_s) / ref.one;
   };
-  float s = sum();
-  if (TAIL && s < 1e-30f) {  // the largest is a listed one, far above all others: again, from the largest of those
+  double s = sum();
+  if (TAIL && s < 1e-30) {  // the largest is a listed one, far above all others: again, from the largest of those
     if constexpr (NT != 64) __syncthreads();
     m = largest();
     s = sum();
@@ -1072,7 +1089,7 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
     finish_distill<NT>(a, row, te[g], TAIL && !twice[g], m, s, tmp_l);
   } else if (t == 0) {
     a.part_sums[index * 2] = m;
-    a.part_sums[index * 2 + 1] = s;
+    a.part_sums[index * 2 + 1] = (float)s;
   }
 }
 

@@ -767,3 +767,28 @@ def test_saved_tensors_that_come_back_packed(cuda, rows, vocab):
         got = step()
     assert torch.equal(got, want)
     assert vocab == 1 or want.abs().sum() > 0
+
+
+@pytest.mark.parametrize('tail', [False, True])
+@pytest.mark.parametrize('vocab, k', [(1, 1), (2, 2), (3, 3), (3, 2), (9, 4), (33, 33), (64, 20)])
+def test_nearly_equal_distributions(cuda, vocab, k, tail):
+    """Few classes, a student that has nearly learnt its teacher: the loss is 1e-4 and less, and right relative to its terms.
+
+    Tolerance, relative to sum q |log q - log p|: e^(v - log norm) 2^-21 (an argument of up to 16) and 2^-22, the logarithms'
+    difference and the product 2^-24 each, a sum of up to 64 terms over lanes 7 * 2^-24: less than 2^-19 together.  The bucket
+    is rounded to fp32: its own 2^-24, and that of the product with its logarithm."""
+    x = logits_of(512, vocab, torch.float32, seed=4)
+    noise = torch.randn(512, vocab, generator=torch.Generator().manual_seed(5)).to(cuda) * 0.01
+    best = token_logprobs(x + noise, top=k)
+    loss = distill_top_logits(x, best.top_indices, best.top_logprobs, tail=tail).double()
+    logp = torch.log_softmax(x.double(), 1)
+    v, lp = best.top_logprobs.double(), logp.gather(1, best.top_indices)
+    log_q = v if tail else v - torch.logsumexp(v, 1, keepdim=True)
+    terms = log_q.exp() * (log_q - lp)
+    want, tol = terms.sum(1), 2.0 ** -19 * terms.abs().sum(1) + 1e-14
+    if tail and k < vocab:
+        rest = (1 - log_q.exp().sum(1)).clamp_min(0)
+        p_o = logp.exp().scatter(1, best.top_indices, 0).sum(1)
+        last = torch.where(rest > 0, rest * (rest.clamp_min(1e-300).log() - p_o.log()), torch.zeros_like(rest))
+        want, tol = want + last, tol + 2.0 ** -19 * last.abs() + 2.0 ** -23 * rest
+    assert ((loss - want).abs() <= tol).all(), ((loss - want).abs() / tol).max()
