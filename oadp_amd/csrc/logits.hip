@@ -978,7 +978,7 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a, int64_t row
 // over the places outside the list is what is kept (1 - sum of the listed p would lose it to rounding), the listed places
 // being known by the bits of a map in LDS: vectors first (a vector's bits are a byte, or half of one), then the single ones.
 // Bound by memory: 4096 x 49408 bf16, 64 entries, 83 us = 4.9 TB/s; 1024 x 100003 fp32 with the bucket, in four chunks a row,
-// 69 + 8.6 for the join = 5.3; 2400 x 1203 fp16 8.5, 300 x 65 5.2: there the list's exponentials and logarithms in 64 bits,
+// 69 + 9.9 for the join = 5.2; 2400 x 1203 fp16 with the bucket 10.2, 300 x 65 5.6: there the list's exponentials and logarithms in 64 bits,
 // one after the other.
 template <typename T, int NT, int NV, bool TAIL, int LIST>
 __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(DistillArgs a) {
