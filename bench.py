@@ -559,7 +559,7 @@ METRIC = {'globals': 'OAKE images/sec (ViT-B/32, 224^2, bs256)',
 
 def _kernel_profile(model, work, one_lane_ms: float | None, n_steps: int) -> tuple[dict, dict, dict]:
     """Per-kernel durations of one step: every launch stamped with the kernel's own begin / end on the launch
-    stream (hipExtLaunchKernelGGL events), one lane, averaged over `n_steps` steps after one warm step under the
+    stream (hipExtLaunchKernelGGL events), one lane, averaged over `n_steps` steps after warm steps under the
     same instrumentation.  The wall clock of those very steps is taken too: the durations must add up to no more
     than it (kernels of one stream do not overlap), and it is printed beside the un-instrumented one-lane step.
     (Round 3 also tried stamping only every S-th launch, so that a stamped kernel runs behind un-instrumented
@@ -569,15 +569,27 @@ def _kernel_profile(model, work, one_lane_ms: float | None, n_steps: int) -> tup
     import torch
     v = model.visual
     v.profile(True)
-    work.step(model)  # warm step under instrumentation, not recorded
-    v.profile(True)   # (resets the slots)
-    torch.cuda.synchronize()
-    t0 = time.perf_counter()
-    for _ in range(n_steps):
+    work.step(model)  # a step under instrumentation, not recorded
+    per_step = sum(p['launches'] for p in v.profile_read())
+    # In groups of a few steps, the stamps read in between: a run of stamps that is longer than any before it lengthens the
+    # kernels while the runtime's event pool grows (objects, 2 images x 40 proposals, 59 launches a step: 41 steps in one run
+    # sum to 3.74 .. 4.44 ms a step, in groups of 4 to 3.47, time after time, beside an un-instrumented step of 3.57).
+    group = max(1, 240 // max(1, per_step))
+    for _ in range(min(group, n_steps)):  # (the pool for a group)
         work.step(model)
-    torch.cuda.synchronize()
-    stamped_wall_ms = (time.perf_counter() - t0) / n_steps * 1e3
-    prof = [p for p in v.profile_read() if p['launches'] > 0]
+    v.profile(True)   # (resets the slots)
+    wall = done = 0
+    while done < n_steps:
+        n = min(group, n_steps - done)
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        for _ in range(n):
+            work.step(model)
+        torch.cuda.synchronize()
+        wall += time.perf_counter() - t0
+        done += n
+        prof = [p for p in v.profile_read() if p['launches'] > 0]  # (adds up over the groups)
+    stamped_wall_ms = wall / n_steps * 1e3
     v.profile(False)
     for p in prof:
         p['ms_per_step'] = p['total_ms'] / n_steps

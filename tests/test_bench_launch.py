@@ -103,3 +103,39 @@ def test_gpus_8_plumbing_eight_gloo_ranks():
     assert line['n_gpus'] == 8 and line['steps'] == 2 and line['scaling'] == 'weak'
     assert 'images x8' in line['config']['sharding'] and 'ranks gathered: 8' in line['config']['sharding']
     assert line['value'] is None and line['cpu_baseline'] is None
+
+
+@pytest.mark.parametrize('launches, n_steps', [(59, 41), (59, 2), (300, 3), (7, 1), (40, 40)])
+def test_stamps_come_in_runs_the_runtime_has_seen(launches, n_steps, monkeypatch):
+    """A run of stamps that is longer than any before it lengthens the kernels it stamps: what is recorded is not one."""
+    import torch
+
+    import bench
+
+    class Visual:
+        longest = pending = total = 0
+
+        def profile(self, enable):
+            self.read()
+            self.total = self.count = 0
+
+        def read(self):
+            self.total += self.pending * (1.25 if self.pending > self.longest else 1.0) * 1e-3
+            self.count = getattr(self, 'count', 0) + self.pending
+            self.longest, self.pending = max(self.longest, self.pending), 0
+
+        def profile_read(self):
+            self.read()
+            return [dict(name='gemm', total_ms=self.total, flops=1e9 * max(1, self.count), bytes=0, launches=self.count)]
+
+    class Model:
+        visual = Visual()
+
+    class Work:
+        def step(self, model):
+            model.visual.pending += launches
+
+    monkeypatch.setattr(torch.cuda, 'synchronize', lambda *a: None)
+    _, kernels, timing = bench._kernel_profile(Model(), Work(), None, n_steps)
+    assert kernels['gemm']['launches_per_step'] == launches == timing['launches_per_step']
+    assert abs(timing['kernels_sum_ms_per_step'] - launches * 1e-3) < 1e-4
