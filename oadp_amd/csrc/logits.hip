@@ -328,6 +328,14 @@ struct Sums {
     s += e;
     t = __builtin_fmaf(e, d, t);
   }
+  // From the fused form to d relative to m.  The product is rounded by itself, as that of a single place's term was (the
+  // compiler would make one operation of the two): a row of one place has t = 0, entropy 0.
+  __device__ __forceinline__ void relative_to_m(const Ref& ref) {
+#pragma clang fp contract(off)
+    const float shift = ref.r * s;
+    t = (t - shift) / ref.one;
+    s /= ref.one;
+  }
 };
 
 // log p of one place, given its logit: -inf where the row holds nothing there
@@ -612,9 +620,8 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void score_kernel(ScoreArgs
     });
     sums.add((tile.single - m) * ref.c);
     reduce();
-  } else {  // relative to m
-    sums.s /= ref.one;
-    sums.t = sums.t / ref.one - ref.r * sums.s;
+  } else {
+    sums.relative_to_m(ref);
   }
 
   RowStats st;

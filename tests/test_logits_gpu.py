@@ -792,3 +792,18 @@ def test_nearly_equal_distributions(cuda, vocab, k, tail):
         last = torch.where(rest > 0, rest * (rest.clamp_min(1e-300).log() - p_o.log()), torch.zeros_like(rest))
         want, tol = want + last, tol + 2.0 ** -19 * last.abs() + 2.0 ** -23 * rest
     assert ((loss - want).abs() <= tol).all(), ((loss - want).abs() / tol).max()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab', [1, 2, 65, 1203, 3001, 9000, 49408, 140001])
+def test_a_single_place_leaves_nothing_open(cuda, vocab, dtype):
+    """One place with a probability: entropy and log probability are 0, not about 0."""
+    at = vocab // 2
+    x = logits_of(40, vocab, dtype, seed=11)
+    mask = torch.zeros(vocab, dtype=torch.bool, device=cuda)
+    mask[at] = True
+    alone = x.masked_fill(~mask, -INF)
+    t = torch.full((40,), at, device=cuda)
+    for scale in (1.0, 0.7, 100.0):
+        for out in (token_logprobs(x, t, top=2, mask=mask, scale=scale), token_logprobs(alone, t, top=2, scale=scale)):
+            assert (out.entropy == 0).all() and (out.logprobs == 0).all() and (out.top_logprobs[:, 0] == 0).all()
