@@ -873,11 +873,14 @@ __device__ __forceinline__ double exp64(double v) {
   for (int k = 11; k > 0; --k) p = __builtin_fma(p * (1.0 / k), r, 1.0);
   return v < -200.0 ? 0.0 : __builtin_ldexp(p, (int)n);
 }
-// log s in 64 bits: that of s in fp32, and one step of Newton's on e^y = s (which squares its error of 2^-24).
+// log s in 64 bits: that of s in fp32, and one step of Newton's on e^y = s (which squares its error of 2^-24).  log 1 = 0: the
+// part that the exponent leaves lies around 1.
 __device__ __forceinline__ double log64(double s) {
   if (s == 0) return -__builtin_inf();
-  const int n = __builtin_amdgcn_frexp_exp(s);
-  const double part = __builtin_ldexp(s, -n), y = logf((float)part);
+  int n = __builtin_amdgcn_frexp_exp(s);
+  double part = __builtin_ldexp(s, -n);
+  if (part < 0.70710678) part += part, n -= 1;
+  const double y = logf((float)part);
   return y + (part * exp64(-y) - 1.0) + n * 0.69314718055994531;
 }
 // By one wave (every lane of it), for the group.  `id`, `v`: the lane's first entry (teacher_entry), fetched before the row

@@ -807,3 +807,20 @@ def test_a_single_place_leaves_nothing_open(cuda, vocab, dtype):
     for scale in (1.0, 0.7, 100.0):
         for out in (token_logprobs(x, t, top=2, mask=mask, scale=scale), token_logprobs(alone, t, top=2, scale=scale)):
             assert (out.entropy == 0).all() and (out.logprobs == 0).all() and (out.top_logprobs[:, 0] == 0).all()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab, n', [(1, 1), (2, 1), (65, 1), (65, 70), (3001, 1), (9000, 1), (140001, 1)])
+def test_a_single_place_has_nothing_to_learn(cuda, vocab, n, dtype):
+    """A student with one place and a teacher that lists it: loss and gradient are 0, not about 0."""
+    at = vocab // 2
+    x = logits_of(40, vocab, dtype, seed=11)
+    x[:, :at] = x[:, at + 1:] = -INF
+    ids = torch.full((40, n), -1, device=cuda)
+    ids[:, n // 2] = at
+    for scale in (1.0, 0.7, 100.0):
+        for tail, v in ((True, 0.0), (False, 0.0), (False, -3.7)):
+            leaf = x.clone().requires_grad_()
+            loss = distill_top_logits(leaf, ids, torch.full((40, n), v, device=cuda), scale=scale, tail=tail)
+            grad, = torch.autograd.grad(loss.sum(), [leaf])
+            assert (loss == 0).all() and (grad == 0).all()
