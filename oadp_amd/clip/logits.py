@@ -152,7 +152,9 @@ def _score(x, targets, mask, mask_stride, top, scale, stats):
 # The backward passes run in torch's device thread, where the same Python takes two to four times as long as in the caller's:
 # what does not depend on the gradients is put together by the forward pass (``ctx.more``), and the launch stands in place
 # (300 x 65, loss and gradient: 97 us with helpers, 86 without; 45 in one thread either way).  Strides are the saved tensors'
-# own: a hook that moves them elsewhere and back (torch.autograd.graph.save_on_cpu) may have packed their rows.
+# own: a hook that moves them elsewhere and back (torch.autograd.graph.save_on_cpu) may have packed their rows.  The
+# gradient's are dense whatever the logits' are (for rows that overlap, empty_like by itself would have others).
+_DENSE = torch.contiguous_format
 
 
 class _TokenLogprobs(torch.autograd.Function):
@@ -188,7 +190,7 @@ class _TokenLogprobs(torch.autograd.Function):
         if mask is not None and mask.dim() == 2:
             mask = mask if mask.stride(1) == 1 else mask.contiguous()
             mask_stride = mask.stride(0)
-        grad = torch.empty_like(x)  # (its rows are dense)
+        grad = torch.empty_like(x, memory_format=_DENSE)
         rc = entry(x.data_ptr(), dtype, rows, vocab, x.stride(0), scale, _ptr(mask), mask_stride, _ptr(targets), index, n,
                    _ptr(top_ids), top, stats.data_ptr(), _ptr(g_logprobs), _ptr(g_lse), _ptr(g_entropy), _ptr(g_top),
                    grad.data_ptr(), vocab, _current_stream(dev))
@@ -274,7 +276,7 @@ class _DistillTopLogits(torch.autograd.Function):
             g_loss = _f32(g_loss)
         if x.stride(1) != 1:
             x = x.contiguous()
-        grad = torch.empty_like(x)
+        grad = torch.empty_like(x, memory_format=_DENSE)
         rc = entry(x.data_ptr(), dtype, rows, vocab, x.stride(0), scale, ids.data_ptr(), index, v.data_ptr(), k, tail,
                    stats.data_ptr(), g_loss.data_ptr(), grad.data_ptr(), vocab, _current_stream(dev))
         if rc:

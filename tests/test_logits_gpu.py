@@ -824,3 +824,30 @@ def test_a_single_place_has_nothing_to_learn(cuda, vocab, n, dtype):
             loss = distill_top_logits(leaf, ids, torch.full((40, n), v, device=cuda), scale=scale, tail=tail)
             grad, = torch.autograd.grad(loss.sum(), [leaf])
             assert (loss == 0).all() and (grad == 0).all()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows, vocab, step', [(4, 9, 1), (7, 9, 2), (5, 65, 1), (6, 1203, 1), (3, 9000, 1), (3, 140001, 1)])
+def test_gradients_of_rows_that_overlap(cuda, rows, vocab, step, dtype):
+    """Sliding windows over one buffer: every row's gradient is what a copy's is, bit for bit."""
+    buf = logits_of(1, vocab + (rows - 1) * step, dtype, seed=12)[0]
+    views = [buf.unfold(0, vocab, step), buf.as_strided((rows, vocab), (step, 1))]
+    allowed = (torch.arange(vocab + rows, device=cuda) % 3 > 0).unfold(0, vocab, 1)[:rows]
+    t = some_targets(rows, vocab, 2)
+    ids, v = a_teacher(rows, vocab, min(8, vocab))
+    up = torch.rand(rows, generator=torch.Generator().manual_seed(0)).to(cuda) + 0.5
+    for view in views:
+        assert view.shape == (rows, vocab) and view.stride() == (step, 1)
+        grads = []
+        for x in (view, view.clone(memory_format=torch.contiguous_format)):
+            leaf = x.detach().requires_grad_()
+            a = token_logprobs(leaf, t, top=3, mask=allowed)
+            loss = distill_top_logits(leaf, ids, v, scale=0.5, tail=True)
+            grads.append((*torch.autograd.grad([a.logprobs, a.entropy, a.top_logprobs], [leaf],
+                                               [up[:, None].expand(rows, 2), up, up[:, None].expand(rows, 3)]),
+                          *torch.autograd.grad([loss], [leaf], [up])))
+        for ours, copy in zip(*grads):
+            assert torch.equal(ours, copy) and copy.abs().sum() > 0
+        want, tol = Score(view, t, 3, mask=allowed).grad(g_logprobs=up[:, None].expand(rows, 2), g_entropy=up,
+                                                         g_top=up[:, None].expand(rows, 3))
+        close(grads[0][0], want, tol)
