@@ -921,7 +921,8 @@ struct DistillArgs {
   float* part_sums;  // [rows, parts, 2]: m, S of a chunk (tail: of its places outside the list)
 };
 // What the backward pass needs of a row: m, 1 / S (0: the student has nothing); the same outside the list; the student's
-// probability there; the teacher's log_norm, q_sum (-1: no entry) and bucket
+// probability there; the teacher's log_norm, q_sum (-1: no entry) and, with the tail, bucket - without (log_norm is 0 with it),
+// what log_norm's rounding left: a list may stand at any height, and 2^-24 of it would be a factor of all its q
 constexpr int kStats = 8;
 constexpr int kExactPlaces = 64;  // rows of so many are summed in 64 bits (few classes: a loss of 1e-4 and less is ordinary)
 __device__ __forceinline__ void write_no_teacher(const DistillArgs& a, int64_t row) {
@@ -978,9 +979,10 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a, int64_t row
     st[2] = mo;
     st[3] = so == 0 ? 0.f : (float)(1 / so);
     st[4] = p_o;
-    st[5] = (float)te.t.log_norm;
+    const float norm = (float)te.t.log_norm;
+    st[5] = norm;
     st[6] = te.t.q_sum;
-    st[7] = rest;
+    st[7] = a.t.tail ? rest : (float)(te.t.log_norm - norm);
   }
 }
 
@@ -1277,14 +1279,15 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_grad_kernel(Di
   int* id = ids[NT == 64 ? threadIdx.x / 64 : 0];
   float* w = ws[NT == 64 ? threadIdx.x / 64 : 0];
   const float* st = a.stats + row * kStats;
-  const float m = st[0], inv_s = st[1], mo = st[2], inv_so = st[3], p_o = st[4], log_norm = st[5], q_sum = st[6], rest = st[7];
+  const float m = st[0], inv_s = st[1], mo = st[2], inv_so = st[3], p_o = st[4], log_norm = st[5], q_sum = st[6];
+  const float rest = a.t.tail ? st[7] : 0.f, norm_rest = a.t.tail ? 0.f : st[7];
   if (q_sum == -1.f || inv_s == 0.f) {
     write_dense<T, NT, NV>(tile, g, a.write_past, [](float) { return 0.f; });
     return;
   }
   for (int i = group_tid<NT>(); i < a.t.n; i += NT) {
     int j;
-    w[i] = expf(teacher_entry(a.t, row, a.r.vocab, i, j) - log_norm);
+    w[i] = expf(teacher_entry(a.t, row, a.r.vocab, i, j) - log_norm - norm_rest);
     id[i] = j;
   }
   const float up = a.g_loss[row] * a.r.scale, c = a.r.scale * kLog2e;

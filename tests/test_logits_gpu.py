@@ -851,3 +851,19 @@ def test_gradients_of_rows_that_overlap(cuda, rows, vocab, step, dtype):
         want, tol = Score(view, t, 3, mask=allowed).grad(g_logprobs=up[:, None].expand(rows, 2), g_entropy=up,
                                                          g_top=up[:, None].expand(rows, 3))
         close(grads[0][0], want, tol)
+
+
+@pytest.mark.parametrize('shift', [0.0, 30.0, -300.0, 1e3, -1e5])
+@pytest.mark.parametrize('vocab, k', [(65, 8), (1203, 64), (5000, 200), (140001, 100)])
+def test_teachers_up_to_a_constant(cuda, vocab, k, shift):
+    """A renormalised list may stand at any height: loss and gradient are those of its differences.  (The reference takes the
+    shifted entries as they came out in fp32, less the shift: exact in 64 bits.)"""
+    x = logits_of(6, vocab, torch.float32, seed=13).requires_grad_()
+    ids, v = a_teacher(6, vocab, k)
+    v = v + shift
+    up = torch.rand(6, generator=torch.Generator().manual_seed(0)).to(cuda) + 0.5
+    loss = distill_top_logits(x, ids, v)
+    grad, = torch.autograd.grad([loss], [x], [up])
+    Distill(x, ids, v.double() - shift).check(loss, grad, up)
+    # p and q both sum to 1: each of the 2 k terms p_j - q_j and the sum of the others is off by 16 steps of its size at most
+    assert (grad.double().sum(1).abs() <= 32 * E * 2 * up).all()
