@@ -854,8 +854,8 @@ __device__ __forceinline__ float teacher_entry(const TeacherArgs& a, int64_t row
 // q = e^(v - log_norm): the softmax of the row's entries, or (tail) e^v as they are and a bucket for what is left of 1,
 // a difference from 1 that is taken in 64 bits
 struct Teacher {
-  double log_norm;
-  float q_sum, q_rest;
+  double log_norm, q_rest;
+  float q_sum;
   bool some;  // there is an entry at all
 };
 template <int CAP>
@@ -909,7 +909,7 @@ __device__ __forceinline__ void teacher_row(const TeacherArgs& a, int64_t row, i
   float q_sum = 0.f;
   for (int i = lane; i < a.n; i += 64) q_sum += expf((float)(s.v[i] - log_norm));
   q_sum = wave64_sum(q_sum);
-  if (lane == 0) s.t = {log_norm, q_sum, a.tail ? (float)(sum > 1 ? 0 : 1 - sum) : 0.f, some != 0.f};
+  if (lane == 0) s.t = {log_norm, a.tail && !(sum > 1) ? 1 - sum : 0, q_sum, some != 0.f};
 }
 
 // ---- distill_top_logits -----------------------------------------------------------------------------------------
@@ -932,10 +932,14 @@ __device__ __forceinline__ void write_no_teacher(const DistillArgs& a, int64_t r
 
 // The end of a row, by one group: `m` and `s` are the row's largest logit and sum (tail: of the places outside the list;
 // the listed ones are added here, each place once).  Where teacher and student nearly agree the loss is a difference of equal
-// logarithms: those, the list's sums and (short rows) all sums are taken in 64 bits.
-template <int NT, int CAP>
+// logarithms: those, the list's sums and (short rows) all sums are taken in 64 bits.  EXACT: so are the terms and their sum
+// (weights and the bucket in fp32 leave the loss off by 2^-24 of the terms, 2e-5 of a loss of 1e-4; 300 x 65 5.3 us without,
+// 5.6 with); not in long rows, whose fp32 sum leaves more than that in log S (4096 x 49408 91 / 95).
+template <int NT, bool EXACT, int CAP>
 __device__ __forceinline__ void finish_distill(const DistillArgs& a, int64_t row, const TeacherList<CAP>& te, bool distinct,
-                                               float m, double s, float* tmp) {
+                                               float m, double s,
+                                               std::conditional_t<EXACT, double, float>* tmp) {
+  using F = std::conditional_t<EXACT, double, float>;
   const int t = group_tid<NT>(), n = a.t.n;
   const float scale = a.r.scale, mo = m;
   const double so = s;
@@ -960,19 +964,22 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a, int64_t row
     p_o = (float)(outside / s);
   }
   const double log_s = log64(s);
-  float loss = 0.f;
+  F loss = 0;
   for (int i = t; i < n; i += NT) {
-    const float v = te.v[i], q = expf((float)(v - te.t.log_norm));
-    if (q == 0.f) continue;
-    const float y = te.id[i] < 0 ? v : te.x[i];  // (an id that the vocabulary does not have: v is NaN)
-    const float lost = y == -kInf && s == s ? kInf : (float)((double)v - te.t.log_norm - ((double)y - m) * scale + log_s);
-    loss += q * lost;
+    const double v = te.v[i], log_q = v - te.t.log_norm;
+    F q;
+    if constexpr (EXACT) q = exp64(log_q);
+    else q = expf((float)log_q);
+    if ((float)q == 0.f) continue;
+    const double y = te.id[i] < 0 ? v : te.x[i];  // (an id that the vocabulary does not have: v is NaN)
+    loss += q * (y == -kInf && s == s ? (F)kInf : (F)(log_q - (y - m) * scale + log_s));
   }
   loss = group_sum<NT>(loss, tmp);
   if (t == 0) {
-    const float rest = !a.t.tail || so == 0 ? 0.f : te.t.q_rest;
-    if (rest != 0.f) loss += rest * (float)(log64(rest) - ((double)mo - m) * scale - log64(so) + log_s);
-    a.loss[row] = loss;
+    const double q_rest = !a.t.tail || so == 0 ? 0 : te.t.q_rest;
+    if (q_rest != 0) loss += (F)q_rest * (F)(log64(q_rest) - ((double)mo - m) * scale - log64(so) + log_s);
+    const float rest = (float)q_rest;
+    a.loss[row] = (float)loss;
     float* st = a.stats + row * kStats;
     st[0] = m;
     st[1] = s == 0 ? 0.f : (float)(1 / s);
@@ -998,7 +1005,9 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
   __shared__ TeacherList<LIST> te[G];
   __shared__ unsigned map[G][WORDS];
   __shared__ int twice[G];
-  __shared__ float tmp_m[NT / 64], tmp_s[NT / 64], tmp_l[NT / 64];
+  __shared__ float tmp_m[NT / 64], tmp_s[NT / 64];
+  constexpr bool EXACT = NT <= 256;
+  __shared__ std::conditional_t<EXACT, double, float> tmp_l[NT / 64];
   const int64_t index = group_index<NT>();
   if (index >= a.r.rows * a.sp.parts) return;
   const int64_t row = a.sp.parts == 1 ? index : index / a.sp.parts;
@@ -1098,7 +1107,7 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
     s = sum();
   }
   if (whole) {
-    finish_distill<NT>(a, row, te[g], TAIL && !twice[g], m, s, tmp_l);
+    finish_distill<NT, EXACT>(a, row, te[g], TAIL && !twice[g], m, s, tmp_l);
   } else if (t == 0) {
     a.part_sums[index * 2] = m;
     a.part_sums[index * 2 + 1] = (float)s;
@@ -1132,7 +1141,7 @@ __global__ __launch_bounds__(kThreads) void distill_join_kernel(DistillArgs a) {
   for (int i = t % 64; i < parts; i += 64)
     if (p[i * 2 + 1] != 0.f) s += p[i * 2 + 1] * __builtin_amdgcn_exp2f((p[i * 2] - m) * (a.r.scale * kLog2e));
   s = wave64_sum(s);
-  finish_distill<kThreads>(a, row, te, false, m, s, tmp);
+  finish_distill<kThreads, false>(a, row, te, false, m, s, tmp);
 }
 
 // ---- gradients --------------------------------------------------------------------------------------------------

@@ -867,3 +867,29 @@ def test_teachers_up_to_a_constant(cuda, vocab, k, shift):
     Distill(x, ids, v.double() - shift).check(loss, grad, up)
     # p and q both sum to 1: each of the 2 k terms p_j - q_j and the sum of the others is off by 16 steps of its size at most
     assert (grad.double().sum(1).abs() <= 32 * E * 2 * up).all()
+
+
+def nearly_equal(vocab, k, pad, tail, rows=512):
+    """(loss, 64-bit loss) of a student that has nearly learnt its teacher; lists padded to k + pad."""
+    x = logits_of(rows, vocab, torch.float32, seed=4)
+    noise = torch.randn(rows, vocab, generator=torch.Generator().manual_seed(5)).cuda() * 0.01
+    best = token_logprobs(x + noise, top=k)
+    ids = torch.nn.functional.pad(best.top_indices, (0, pad), value=-1)
+    loss = distill_top_logits(x, ids, torch.nn.functional.pad(best.top_logprobs, (0, pad), value=-INF), tail=tail).double()
+    logp = torch.log_softmax(x.double(), 1)
+    v, lp = best.top_logprobs.double(), logp.gather(1, best.top_indices)
+    log_q = v if tail else v - torch.logsumexp(v, 1, keepdim=True)
+    terms = log_q.exp() * (log_q - lp)
+    if tail and k < vocab:
+        rest = (1 - log_q.exp().sum(1, keepdim=True)).clamp_min(0)
+        p_o = logp.exp().scatter(1, best.top_indices, 0).sum(1, keepdim=True)
+        terms = torch.cat([terms, torch.where(rest > 0, rest * (rest.clamp_min(1e-300).log() - p_o.log()), torch.zeros_like(rest))], 1)
+    return loss, terms.sum(1)
+
+
+@pytest.mark.parametrize('tail', [False, True])
+@pytest.mark.parametrize('vocab, k', [(2, 1), (3, 3), (9, 4), (13, 1), (23, 5), (33, 33), (52, 50), (64, 20)])
+def test_small_losses_have_all_their_digits(cuda, vocab, k, tail):
+    """Tolerance: the loss is rounded once, 2^-24 of it, doubled; e^y in 64 bits is off by 1e-13 of terms of 1e-2."""
+    loss, want = nearly_equal(vocab, k, 0, tail)
+    assert ((loss - want).abs() <= 2.0 ** -23 * want.abs() + 1e-14).all(), ((loss - want) / want).abs().max()
