@@ -924,7 +924,10 @@ struct DistillArgs {
 // probability there; the teacher's log_norm, q_sum (-1: no entry) and, with the tail, bucket - without (log_norm is 0 with it),
 // what log_norm's rounding left: a list may stand at any height, and 2^-24 of it would be a factor of all its q
 constexpr int kStats = 8;
-constexpr int kExactPlaces = 64;  // rows of so many are summed in 64 bits (few classes: a loss of 1e-4 and less is ordinary)
+// Rows of so many are summed in 64 bits, whoever works on them (few classes: a loss of 1e-4 and less is ordinary).  fp32 /
+// 64 bits, us: 300 x 65 fp32 5.6 / 6.0, 19200 x 65 fp32 21 / 26, fp16 (eight places a lane) 21 / 30, x 128 fp16 20 / 30.  A detector's 65 classes
+// are well inside; longer rows keep what their fp32 sum leaves in log S.
+constexpr int kExactPlaces = 128;
 __device__ __forceinline__ void write_no_teacher(const DistillArgs& a, int64_t row) {
   a.loss[row] = 0.f;
   a.stats[row * kStats + 6] = -1.f;
@@ -1006,7 +1009,8 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
   __shared__ unsigned map[G][WORDS];
   __shared__ int twice[G];
   __shared__ float tmp_m[NT / 64], tmp_s[NT / 64];
-  constexpr bool EXACT = NT <= 256;
+  constexpr bool EXACT = NT <= 256;  // (workgroups of 512 have longer rows)
+  __shared__ double tmp_d[NT / 64];
   __shared__ std::conditional_t<EXACT, double, float> tmp_l[NT / 64];
   const int64_t index = group_index<NT>();
   if (index >= a.r.rows * a.sp.parts) return;
@@ -1073,15 +1077,15 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
     const Ref ref(m, a.r.scale * kLog2e);
     m = ref.m;
     tile.pack();
-    if constexpr (NT == 64) {
-      if (tile.n <= kExactPlaces) {
+    if constexpr (EXACT) {
+      if (whole && tile.n <= kExactPlaces) {
         const auto e = [&](float v) { return exp64(((double)v - m) * a.r.scale); };
         double s = e(tile.single);
-        tile.each([&](u32x4_t q, int) {
+        if (tile.has_vec(0)) {  // (nobody has more than one)
 #pragma unroll
-          for (int i = 0; i < E; ++i) s += e(elem<T>(q, i));
-        });
-        return wave64_sum(s);
+          for (int i = 0; i < E; ++i) s += e(elem<T>(tile.v[0], i));
+        }
+        return group_sum<NT>(s, tmp_d);
       }
     }
     float s = 0.f;

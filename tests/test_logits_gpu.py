@@ -893,3 +893,12 @@ def test_small_losses_have_all_their_digits(cuda, vocab, k, tail):
     """Tolerance: the loss is rounded once, 2^-24 of it, doubled; e^y in 64 bits is off by 1e-13 of terms of 1e-2."""
     loss, want = nearly_equal(vocab, k, 0, tail)
     assert ((loss - want).abs() <= 2.0 ** -23 * want.abs() + 1e-14).all(), ((loss - want) / want).abs().max()
+
+
+@pytest.mark.parametrize('tail', [False, True])
+@pytest.mark.parametrize('vocab, k, pad', [(65, 8, 0), (65, 65, 0), (65, 8, 60), (100, 20, 0), (128, 128, 0), (7, 7, 93), (7, 3, 1000),
+                                           (2, 2, 63), (64, 20, 280), (128, 100, 0)])
+def test_sums_of_short_rows_whatever_the_list(cuda, vocab, k, pad, tail):
+    """Rows of up to 128 places have the same digits whatever the length of the list.  Tolerance as above."""
+    loss, want = nearly_equal(vocab, k, pad, tail)
+    assert ((loss - want).abs() <= 2.0 ** -23 * want.abs() + 1e-14).all(), ((loss - want) / want).abs().max()
