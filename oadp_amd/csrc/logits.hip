@@ -1316,16 +1316,18 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_grad_kernel(Di
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------
-// Who works on a row, by its length alone: a wave where its registers hold the row (four rows a workgroup, no barriers; by
+// Who works on a row, by its length and its lists': a wave where its registers hold the row (four rows a workgroup, no barriers; by
 // wave / 256 threads, us: 300 x 65 fp32, 5 alternatives 4.7 / 9.7, 16384 x 2000 fp16, 20 23 / 63, 65536 x 1203 62 / 233,
 // its gradient 62 / 100), a workgroup of 256 threads with 8 vectors each, or of 512 with 16 (256 / 512: 2400 x 4500 bf16
 // 11.9 / 26, 8192 x 16000 49 / 93) - beyond that the row is cut into equal chunks, which a second launch joins.  The chunks
 // are as long as they can be, few rows or many: a quarter as long with 256 threads, the join has four times the lists (a
 // quarter / whole, us with the join: 16 x 200003 fp32, 100 alternatives 23 / 19, 20 14.6 / 11.9, 1 x 262143 bf16 11.9 /
 // 12.8, 32 x 131071 bf16 12.3 / 15.6).  Gradients need no join and take 256 threads with 4 vectors (2 or 8: within 5 %).
-// Rows of 2049 .. 4096 places go to a wave with twice the vectors where there are enough of them to fill the device at its
-// half occupancy and few alternatives to look for (wave / workgroup, us: 32768 x 2500 bf16, 20 alternatives 54 / 96;
-// 2400 x 2500 8.1 / 11.3; 1024 x 4000 7.4 / 7.0; 8192 x 4000 fp32, 100 alternatives 61 / 52; 2400 x 4000 fp32, 20 12.9 / 12.7).
+// Rows of 2049 .. 4096 places go to a wave with twice the vectors where there are few alternatives to look for (wave /
+// workgroup, us: 32768 x 2500 bf16, 20 alternatives 54 / 96; 2400 x 2500 8.1 / 11.3; 8192 x 4000 fp32, 100 alternatives 61 / 52;
+// 2000 x 3000 fp16, 20 entries and the bucket 9.7 / 15.2).  That few rows would take less in workgroups (1 x 3000 fp16 5.2 / 4.6,
+// 300 x 4096 fp32 8.1 / 5.7, under calls that the host takes 17 us for) does not count: how many there are decides nothing, so
+// that a row has the same bits in any batch.
 constexpr int kBlockVecs = 8, kLongVecs = 16, kGradVecs = 4;
 constexpr int kWaveList = 64;  // entries of a list that a wave's share of the LDS holds
 struct Plan {
@@ -1338,15 +1340,15 @@ Split split(int64_t vocab, int64_t most) {  // equal chunks of at most `most` pl
   const int64_t parts = (vocab + most - 1) / most, chunk = ((vocab + parts - 1) / parts + 7) / 8 * 8;
   return {chunk, (int)((vocab + chunk - 1) / chunk)};
 }
-Plan forward_plan(int64_t rows, int64_t vocab, int dtype, int top, int list) {
+Plan forward_plan(int64_t vocab, int dtype, int top, int list) {
   if (list <= kWaveList) {
     if (vocab <= kWavePlaces) return {64, false, {vocab, 1}};
-    if (vocab <= 2 * kWavePlaces && rows >= 2048 && top <= 32) return {64, true, {vocab, 1}};
+    if (vocab <= 2 * kWavePlaces && top <= 32) return {64, true, {vocab, 1}};
   }
   if (vocab <= capacity(256, kBlockVecs, dtype)) return {256, false, {vocab, 1}};
   return {512, false, split(vocab, capacity(512, kLongVecs, dtype))};
 }
-Plan backward_plan(int64_t rows, int64_t vocab, int dtype, int list) {
+Plan backward_plan(int64_t vocab, int dtype, int list) {
   if (vocab <= kWavePlaces && list <= kWaveList) return {64, false, {vocab, 1}};
   return {256, false, split(vocab, capacity(256, kGradVecs, dtype))};
 }
@@ -1479,7 +1481,7 @@ int oake_logits_workspace(int64_t rows, int64_t vocab, int dtype, int top, size_
   if (!bytes) return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
   if (int rc = check_rows(what, bytes, dtype, rows, vocab, vocab, 1.f)) return rc;
   if (top < 0 || top > kMaxTop) return refuse(OAKE_ERR_INVALID, "%s: top must be 0 .. %d", what, kMaxTop);
-  *bytes = scratch_bytes(rows, forward_plan(rows, vocab, dtype, top, 0).sp, top);
+  *bytes = scratch_bytes(rows, forward_plan(vocab, dtype, top, 0).sp, top);
   return OAKE_OK;
 }
 
@@ -1495,7 +1497,7 @@ int oake_token_logprobs(const void* d_logits, int dtype, int64_t rows, int64_t v
   if (rows == 0) return OAKE_OK;
   if ((n_targets && (!d_targets || !d_logprobs)) || (top && (!d_top_logprobs || !d_top_indices)))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
-  const Plan p = forward_plan(rows, vocab, dtype, top, 0);
+  const Plan p = forward_plan(vocab, dtype, top, 0);
   if (blocks_of(p, rows) > kMostBlocks) return refuse(OAKE_ERR_INVALID, "%s: too many rows of this length", what);
   if (int rc = check_scratch(what, d_workspace, workspace_bytes, scratch_bytes(rows, p.sp, top))) return rc;
   float* sums = static_cast<float*>(d_workspace);
@@ -1523,7 +1525,7 @@ int oake_token_logprobs_backward(const void* d_logits, int dtype, int64_t rows, 
   if (int rc = check_grad(what, d_grad, dtype, vocab, rows, grad_stride)) return rc;
   if (!d_stats || (d_grad_logprobs && n_targets && !d_targets) || (d_grad_top && top && !d_top_indices))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
-  const Plan p = backward_plan(rows, vocab, dtype, (d_grad_logprobs ? n_targets : 0) + (d_grad_top ? top : 0));
+  const Plan p = backward_plan(vocab, dtype, (d_grad_logprobs ? n_targets : 0) + (d_grad_top ? top : 0));
   if (blocks_of(p, rows) > kMostBlocks) return refuse(OAKE_ERR_INVALID, "%s: too many rows of this length", what);
   const ScoreGradArgs a{{d_logits, rows, vocab, row_stride, d_mask, mask_stride, scale,
                          past_cache(rows, vocab, element_size(dtype), 256 << 20)}, p.sp,
@@ -1543,7 +1545,7 @@ int oake_distill_top_logits(const void* d_logits, int dtype, int64_t rows, int64
   if (rows == 0) return OAKE_OK;
   if (!d_loss || !d_stats || (top && (!d_top_indices || !d_top_logprobs)))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
-  const Plan p = forward_plan(rows, vocab, dtype, 0, top);
+  const Plan p = forward_plan(vocab, dtype, 0, top);
   if (blocks_of(p, rows) > kMostBlocks) return refuse(OAKE_ERR_INVALID, "%s: too many rows of this length", what);
   if (int rc = check_scratch(what, d_workspace, workspace_bytes, scratch_bytes(rows, p.sp, 0))) return rc;
   const DistillArgs a{{d_logits, rows, vocab, row_stride, nullptr, 0, scale,
@@ -1565,7 +1567,7 @@ int oake_distill_top_logits_backward(const void* d_logits, int dtype, int64_t ro
   if (int rc = check_grad(what, d_grad, dtype, vocab, rows, grad_stride)) return rc;
   if (!d_stats || !d_grad_loss || (top && (!d_top_indices || !d_top_logprobs)))
     return refuse(OAKE_ERR_INVALID, "%s: null pointer", what);
-  const Plan p = backward_plan(rows, vocab, dtype, top);
+  const Plan p = backward_plan(vocab, dtype, top);
   if (blocks_of(p, rows) > kMostBlocks) return refuse(OAKE_ERR_INVALID, "%s: too many rows of this length", what);
   const DistillGradArgs a{{d_logits, rows, vocab, row_stride, nullptr, 0, scale,
                            past_cache(rows, vocab, element_size(dtype), 256 << 20)}, p.sp,

@@ -902,3 +902,28 @@ def test_sums_of_short_rows_whatever_the_list(cuda, vocab, k, pad, tail):
     """Rows of up to 128 places have the same digits whatever the length of the list.  Tolerance as above."""
     loss, want = nearly_equal(vocab, k, pad, tail)
     assert ((loss - want).abs() <= 2.0 ** -23 * want.abs() + 1e-14).all(), ((loss - want) / want).abs().max()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab', [65, 1203, 2049, 3000, 4096, 9000, 49408, 140001])
+def test_bits_do_not_depend_on_the_batch(cuda, vocab, dtype):
+    """Every output and gradient of a row is the same, bit for bit, alone, among a few rows and among many."""
+    many = 2100 if vocab < 5000 else 300
+    x = logits_of(many, vocab, dtype, seed=14)
+    t = some_targets(many, vocab, 2)
+    up = torch.rand(many, generator=torch.Generator().manual_seed(0)).to(cuda) + 0.5
+    ids, v = a_teacher(many, vocab, 20)
+
+    def step(rows, top, tail):
+        leaf = x[rows].detach().requires_grad_()
+        n, u = leaf.shape[0], up[rows]
+        a = token_logprobs(leaf, t[rows], top=top, scale=0.9)
+        loss = distill_top_logits(leaf, ids[rows], v[rows], scale=0.5, tail=tail)
+        return [*a, loss, *torch.autograd.grad([a.logprobs, a.entropy], [leaf], [u[:, None].expand(n, 2), u]),
+                *torch.autograd.grad([loss], [leaf], [u])]
+
+    for top, tail in ((20, False), (33, True)):
+        whole = step(slice(0, many), top, tail)
+        for rows in (slice(5, 6), slice(3, 10), slice(0, many - 60)):
+            for name, (a, b) in enumerate(zip(step(rows, top, tail), whole)):
+                assert torch.equal(a, b[rows]), (rows, top, name)
