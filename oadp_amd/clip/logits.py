@@ -21,6 +21,7 @@ from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
@@ -41,13 +42,23 @@ class TokenLogprobs(NamedTuple):
     top_indices: torch.Tensor | None    # [..., top], -1 where there are fewer alternatives
 
 
+def _check_no_tangent(**tensors: torch.Tensor | None) -> None:
+    if getattr(forward_ad, '_current_level', 0) < 0:  # (no level of dual tensors has been entered)
+        return
+    for name, t in tensors.items():
+        if isinstance(t, torch.Tensor) and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f'{name} has a forward-mode tangent, which these operators do not carry on')
+
+
 def _check_scale(scale: float | torch.Tensor) -> float:
+    _check_no_tangent(scale=scale)
     if isinstance(scale, torch.Tensor) and scale.requires_grad and torch.is_grad_enabled():
         raise ValueError('scale gets no gradient: detach() it, or multiply the logits by a learnt scale')
     return float(scale)
 
 
 def _check_logits(logits: torch.Tensor, scale: float) -> None:
+    _check_no_tangent(logits=logits)
     if logits.dtype not in _DTYPES:
         raise TypeError(f'unsupported logits dtype {logits.dtype}')
     if logits.dim() < 1 or logits.shape[-1] < 1:
@@ -210,8 +221,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     (NaN and inf included) is without effect and its gradient is 0.  A row with nothing allowed: lse -inf, entropy 0,
     log probabilities -inf, gradient 0.
 
-    Differentiable once in ``logits`` (not in ``scale``: multiply the logits by a learnt one) through logprobs, entropy,
-    lse and top_logprobs (a log probability of -inf is a constant)."""
+    Differentiable once, backward, in ``logits`` (not in ``scale``: multiply the logits by a learnt one) through logprobs,
+    entropy, lse and top_logprobs (a log probability of -inf is a constant); a forward-mode tangent is refused."""
     scale, top = _check_scale(scale), int(top)
     _check_logits(logits, scale)
     if not 0 <= top <= MAX_TOP:
@@ -296,7 +307,8 @@ def distill_top_logits(logits: torch.Tensor, top_indices: torch.Tensor, top_logp
     from moving its mass out of (or into) the list.  Temperature T: ``scale = 1 / T`` here and for the teacher's call,
     and T^2 times the loss to keep the gradient's size.
 
-    Differentiable once in ``logits``; the teacher and ``scale`` get no gradient."""
+    Differentiable once, backward, in ``logits``; the teacher and ``scale`` get no gradient, a forward-mode tangent is
+    refused."""
     scale, tail = _check_scale(scale), bool(tail)
     _check_logits(logits, scale)
     if top_indices.dtype not in _INDEX:
@@ -312,6 +324,7 @@ def distill_top_logits(logits: torch.Tensor, top_indices: torch.Tensor, top_logp
         raise ValueError(f'at most {MAX_LIST} entries per row, got {k}')
     if top_logprobs.requires_grad and torch.is_grad_enabled():
         raise ValueError('the teacher gets no gradient: detach() its top_logprobs')
+    _check_no_tangent(top_logprobs=top_logprobs)
     _check_same_device(logits, top_indices=top_indices, top_logprobs=top_logprobs)
     x = _as_rows(logits)
     ids, v = top_indices, top_logprobs.detach() if top_logprobs.requires_grad else top_logprobs

@@ -140,3 +140,22 @@ def test_a_learnt_scale_is_refused():
             call(learnt.detach())
         with torch.no_grad(), pytest.raises(RuntimeError, match='GPU'):
             call(learnt)
+
+
+def test_a_forward_mode_tangent_is_refused():
+    """Outputs without a tangent would say that nothing depends on the input."""
+    from torch.autograd import forward_ad as fw
+    with fw.dual_level():
+        dual = fw.make_dual(X.clone(), torch.ones_like(X))
+        lp = fw.make_dual(LP.clone(), torch.ones_like(LP))
+        scale = fw.make_dual(torch.tensor(2.0), torch.tensor(1.0))
+        for call in (lambda: token_logprobs(dual), lambda: token_logprobs(dual.clone().requires_grad_()),
+                     lambda: token_logprobs(X, scale=scale), lambda: distill_top_logits(dual, IDS, LP),
+                     lambda: distill_top_logits(X, IDS, lp), lambda: distill_top_logits(X, IDS, LP, scale=scale)):
+            with pytest.raises(ValueError, match='tangent'):
+                call()
+        for call in (lambda: token_logprobs(X, IDS), lambda: distill_top_logits(X, IDS, LP)):  # no tangent: past the checks
+            with pytest.raises(RuntimeError, match='GPU'):
+                call()
+    with pytest.raises(RuntimeError, match='GPU'):
+        token_logprobs(X)
