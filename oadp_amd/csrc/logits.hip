@@ -10,8 +10,10 @@
 //
 // A row of `vocab` logits x (fp32, fp16 or bf16) and a positive scale give z = scale * x and p = softmax(z).  Everything
 // is kept relative to the row's largest logit m: d = scale * (x - m) <= 0, S = sum e^d, so that log p = d - log S keeps
-// its digits where it is small, whatever the size of m (lse = scale * m + log S is rounded once, at the end).  All of it
-// is fp32; 16 bits appear only in the logits and, rounded once, in their gradient.
+// its digits where it is small, whatever the size of m (lse = scale * m + log S is rounded once, at the end).  Logits,
+// exponentials, sums and gradients are fp32; the distillation loss has 64 bits where it is a difference of nearly equal
+// numbers (the teacher's sum and norm, the logarithms, short rows whole); 16 bits appear only in the logits and, rounded once,
+// in their gradient.
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -347,7 +349,7 @@ __device__ __forceinline__ float logp_at(float x, float m, float log_s, float sc
 // A lower bound of the row's top-th largest logit: of the maxima of (at least top) disjoint parts of the row, about the
 // top-th largest - that many places reach it.  It is looked for by counting over the wave's lanes.  In the pass of the sums
 // the vectors that hold a place at or above it go to LDS as they are, their places there become keys, and each key's rank is
-// the number of larger ones.  49408 normal logits, 256 parts, top 20: about 21 keys.  Where a list overflows (crowded equal
+// the number of larger ones.  49408 normal logits, top 20, of 64 parts' maxima: about 24 keys, 36 at most of 300 rows.  Where a list overflows (crowded equal
 // values) or the row has NaN (which the maxima pass over), the top-th key itself is looked for by counting over the row.
 constexpr float kLowest = -3.402823466e38f;
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }

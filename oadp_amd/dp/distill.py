@@ -19,7 +19,7 @@ class TopLogitsDistillation:
     the teacher's list.  ``scale``: CLIP's logit scale; ``temperature`` T divides the teacher's and the student's logits
     alike, and the loss is multiplied by T^2 so that its gradient keeps its size.  ``tail``: what the list leaves out counts
     as one more outcome (``distill_top_logits``).  ``mask`` (bool [n]): the labels that are taught - the others are left out
-    of the teacher's distribution."""
+    of the teacher's distribution (the student's is over all of them; with ``tail`` they share the bucket)."""
 
     def __init__(self, labels: torch.Tensor, *, top: int = 32, scale: float = 100.0, temperature: float = 1.0,
                  tail: bool = True, mask: torch.Tensor | None = None) -> None:

@@ -159,3 +159,23 @@ def test_a_forward_mode_tangent_is_refused():
                 call()
     with pytest.raises(RuntimeError, match='GPU'):
         token_logprobs(X)
+
+
+def test_refusals_say_why(lib):
+    """The text of a refusal is the library's own and names what was wrong."""
+    buf, n = C.create_string_buffer(4096), C.c_size_t(0)
+    p = C.addressof(buf) + (-C.addressof(buf)) % 64
+
+    def why(rc):
+        with pytest.raises(_lib.OakeError) as e:
+            _lib.check(lib, None, rc, 'a call')
+        return str(e.value)
+
+    assert 'top must be 0 .. 128' in why(lib.oake_logits_workspace(1, 1, _lib.OAKE_F32, 500, C.byref(n)))
+    for scale in (0.0, 1e-60, 2e38):  # (1e-60 is 0 in fp32)
+        assert 'scale must be positive and at most 1e38' in why(lib.oake_token_logprobs(
+            p, _lib.OAKE_F32, 3, 7, 7, scale, None, 0, None, 0, 0, 0, None, p, p, None, None, None, None, 0, None))
+        assert 'scale must be positive and at most 1e38' in why(lib.oake_distill_top_logits(
+            p, _lib.OAKE_F32, 3, 7, 7, scale, p, _lib.OAKE_I64, p, 1, 0, p, p, None, 0, None))
+    assert 'n_targets must be 0 .. 1024' in why(lib.oake_token_logprobs(
+        p, _lib.OAKE_F32, 3, 7, 7, 1.0, None, 0, p, _lib.OAKE_I64, 1025, 0, p, p, p, None, None, None, None, 0, None))
