@@ -927,8 +927,8 @@ struct DistillArgs {
 // what log_norm's rounding left: a list may stand at any height, and 2^-24 of it would be a factor of all its q
 constexpr int kStats = 8;
 // Rows of so many are summed in 64 bits, whoever works on them (few classes: a loss of 1e-4 and less is ordinary).  fp32 /
-// 64 bits, us: 300 x 65 fp32 5.6 / 6.0, 19200 x 65 fp32 21 / 26, fp16 (eight places a lane) 21 / 30, x 128 fp16 20 / 30.  A detector's 65 classes
-// are well inside; longer rows keep what their fp32 sum leaves in log S.
+// 64 bits, us: 300 x 65 fp32 5.6 / 6.0, 19200 x 65 fp32 21 / 26, fp16 (eight places a lane) 21 / 30, x 128 fp16 20 / 30.  A
+// detector's 65 classes are well inside; longer rows keep what their fp32 sum leaves in log S.
 constexpr int kExactPlaces = 128;
 __device__ __forceinline__ void write_no_teacher(const DistillArgs& a, int64_t row) {
   a.loss[row] = 0.f;
@@ -1002,8 +1002,8 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a, int64_t row
 // over the places outside the list is what is kept (1 - sum of the listed p would lose it to rounding), the listed places
 // being known by the bits of a map in LDS: vectors first (a vector's bits are a byte, or half of one), then the single ones.
 // Bound by memory: 4096 x 49408 bf16, 64 entries, 83 us = 4.9 TB/s; 1024 x 100003 fp32 with the bucket, in four chunks a row,
-// 69 + 9.9 for the join = 5.2; 2400 x 1203 fp16 with the bucket 10.2, 300 x 65 5.6: there the list's exponentials and logarithms in 64 bits,
-// one after the other.
+// 69 + 10.2 for the join = 5.1; 2400 x 1203 fp16 with the bucket 10.8, 300 x 65 6.4: there the list's exponentials and logarithms
+// in 64 bits, one after the other.
 template <typename T, int NT, int NV, bool TAIL, int LIST>
 __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(DistillArgs a) {
   constexpr int G = kGroups<NT>, E = kPer<T>, WORDS = TAIL ? NT * NV * E / 32 + 1 : 1;
@@ -1120,7 +1120,9 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_kernel(Distill
   }
 }
 
-// The chunks of a row joined, as above: of the sums, and the loss from the list (whose logits are read here).
+// The chunks of a row joined, as above: of the sums, and the loss from the list (whose logits are read here).  Places listed
+// twice are looked for by comparing each entry with those before it: nothing for 32 entries, most of the time for many
+// (1024 x 100003 fp32 with the bucket, forward: 32 entries 82 us, 128 103, 512 308, 1024 805).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void distill_join_kernel(DistillArgs a) {
   __shared__ TeacherList<kMaxList> te;
@@ -1176,7 +1178,8 @@ __device__ __forceinline__ void write_dense(const Tile<T, NT, NV>& tile, T* g, b
     }
   if (tile.has_single()) g[tile.single_col()] = to16<T>(value(tile.single));
 }
-// the listed places of a chunk; value(x, weight)
+// the listed places of a chunk; value(x, weight).  Each looks through the whole list (1024 x 100003 fp32: 32 entries 146 us, 1024
+// 3106).
 template <typename T, int NT, typename F>
 __device__ __forceinline__ void write_listed(const int* id, const float* w, int n, const T* x, T* g, int64_t first, int count,
                                              F value) {
