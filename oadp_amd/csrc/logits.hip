@@ -349,8 +349,9 @@ __device__ __forceinline__ float logp_at(float x, float m, float log_s, float sc
 // A lower bound of the row's top-th largest logit: of the maxima of (at least top) disjoint parts of the row, about the
 // top-th largest - that many places reach it.  It is looked for by counting over the wave's lanes.  In the pass of the sums
 // the vectors that hold a place at or above it go to LDS as they are, their places there become keys, and each key's rank is
-// the number of larger ones.  49408 normal logits, top 20, of 64 parts' maxima: about 24 keys, 36 at most of 300 rows.  Where a list overflows (crowded equal
-// values) or the row has NaN (which the maxima pass over), the top-th key itself is looked for by counting over the row.
+// the number of larger ones.  49408 normal logits, top 20, of 64 parts' maxima: about 24 keys, 36 at most of 300 rows.  Where
+// a list overflows (crowded equal values) or the row has NaN (which the maxima pass over), the top-th key itself is looked for
+// by counting over the row.
 constexpr float kLowest = -3.402823466e38f;
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ float bound_of(uint32_t prefix) {
