@@ -148,3 +148,13 @@ def test_pass_planner_host_arithmetic(lib):
             per = plan(cap, n, tokens, per_tile, ncu)
             k0 = -(-n // cap)
             assert 1 <= per <= cap and k0 <= -(-n // per) <= k0 + 2, (cap, n, tokens, per, ncu)
+
+
+def test_build_compiles_whatever_is_there(monkeypatch):
+    """``build()`` is the check that everything compiles: sources that have not changed are no exception."""
+    import __graft_entry__
+    from oadp_amd import build
+    asked = []
+    monkeypatch.setattr(build, 'build_library', lambda force=False, **kw: asked.append(force))
+    __graft_entry__.build()
+    assert asked == [True]
