@@ -305,8 +305,9 @@ def distill_top_logits(logits: torch.Tensor, top_indices: torch.Tensor, top_logp
     ``tail=False``: the teacher's entries are renormalised to 1.  ``tail=True``: they are taken as they are, and all
     places outside the list are one more outcome with the teacher's remaining probability, which keeps the student
     from moving its mass out of (or into) the list; that outcome is left out where the student rules out all of those
-    places (-inf), while a listed place that it gives probability 0 makes the loss +inf.  Temperature T: ``scale = 1 / T`` here and for the teacher's call,
-    and T^2 times the loss to keep the gradient's size.
+    places (-inf), while a listed place that it gives probability 0 makes the loss +inf.
+
+    Temperature T: ``scale = 1 / T`` here and for the teacher's call, and T^2 times the loss to keep the gradient's size.
 
     Differentiable once, backward, in ``logits``; the teacher and ``scale`` get no gradient, a forward-mode tangent is
     refused."""

@@ -1322,8 +1322,8 @@ __global__ __launch_bounds__(kBlock<NT>, kWaves<NT>) void distill_grad_kernel(Di
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------
-// Who works on a row, by its length and its lists': a wave where its registers hold the row (four rows a workgroup, no barriers; by
-// wave / 256 threads, us: 300 x 65 fp32, 5 alternatives 4.7 / 9.7, 16384 x 2000 fp16, 20 23 / 63, 65536 x 1203 62 / 233,
+// Who works on a row, by its length and its lists': a wave where its registers hold the row (four rows a workgroup, no
+// barriers; by wave / 256 threads, us: 300 x 65 fp32, 5 alternatives 4.7 / 9.7, 16384 x 2000 fp16, 20 23 / 63, 65536 x 1203 62 / 233,
 // its gradient 62 / 100), a workgroup of 256 threads with 8 vectors each, or of 512 with 16 (256 / 512: 2400 x 4500 bf16
 // 11.9 / 26, 8192 x 16000 49 / 93) - beyond that the row is cut into equal chunks, which a second launch joins.  The chunks
 // are as long as they can be, few rows or many: a quarter as long with 256 threads, the join has four times the lists (a
