@@ -306,8 +306,8 @@ OAKE_API int oake_jpeg_reconstruct(oake_handle* h, const uint8_t* h_data, size_t
  * 1 .. 2^31 - 1.  z = scale * logit with 0 < scale <= 1e38 (CLIP's logit scale, 1 / temperature), p = softmax(z) over
  * the allowed places; sums and statistics are fp32 (oake_distill_top_logits: 64 bits for the teacher's list and its
  * logarithms, and for the whole loss of rows of up to 128 places), gradients rounded once to `dtype`.  Index lists are
- * OAKE_I32 | OAKE_I64, contiguous; a negative index is padding.  An index >= vocab cannot be refused without waiting for the GPU: it is never
- * followed, and makes what depends on it NaN.  All pointers are aligned to their element type.
+ * OAKE_I32 | OAKE_I64, contiguous; a negative index is padding.  An index >= vocab cannot be refused without waiting for
+ * the GPU: it is never followed, and makes what depends on it NaN.  All pointers are aligned to their element type.
  *
  * oake_logits_workspace: bytes of scratch the two forward entry points need for these sizes (often 0; `top` as passed
  * there to oake_token_logprobs, 0 for oake_distill_top_logits).  The workspace is 16-byte aligned, needs no
